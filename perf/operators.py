@@ -434,7 +434,7 @@ def run(state):
             kvq.paged_append(st["k_new"], st["v_new"], st["k"], st["v"], st["ks"], st["vs"], st["table"], st["start"],
                              st["new_lens"], k_zp=st["kz"], v_zp=st["vz"])
             k, v = kvq.paged_read(st["k"], st["v"], st["ks"], st["vs"], st["table"], st["start"], case["T"], st["new_lens"],
-                                  k_zp=st["kz"], v_zp=st["vz"])
+                                  head_dim=case["D"], k_zp=st["kz"], v_zp=st["vz"])
             outs = {"k": k, "v": v}
         else:
             outs = _plain_append(st)
