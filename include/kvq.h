@@ -406,10 +406,130 @@ typedef struct KvqDequantArgs {
 KVQ_API int kvq_dequantize(const KvqDequantArgs* args, kvq_stream_t stream);
 
 /*
+ * ---------------------------------------------------------------- bounded and shared cache memory
+ * The three attention forms below (paged, windowed, weight-accumulating) read the cache formats of kvq_decode_attn.
+ * The value of a cached element is code * scale (+ zero-point), a product that fits 32 bits exactly; no rounding to
+ * fp16 happens on the way into the sums.
+ */
+
+/* Where the tokens of a batch row live.  table == NULL: contiguous, token s at s * stride_s of the row.  Otherwise the
+ * payload / scale / zero-point buffers are pools [num_pages, Hkv, page_size, .] (their stride_b is the PAGE stride) and
+ * token s of row b is row s % page_size of page table[b * stride_b + s / page_size].  Entries behind a row's last token
+ * are never read.  An entry outside [0, num_pages) that would be needed raises bit 3 of kvq_debug_error_flag: an append
+ * stores nothing for that token, attention and read-back use page 0 in its place (memory-safe, the row is meaningless). */
+typedef struct KvqPageTable {
+    const int32_t* table;        /* device int32 [B, cols] or NULL                           */
+    int64_t stride_b;            /* elements                                                 */
+    int32_t cols;                /* pages a row can have                                     */
+    int32_t page_size;           /* tokens per page, > 0                                     */
+    int32_t num_pages;
+} KvqPageTable;
+
+/*
+ * q_len == 1 attention over a visible span of each row:
+ *   visible(b) = { s < n_b : window == 0 or s < sinks or s >= n_b - window },  n_b = context_lens[b] clamped to
+ *   [0, max_ctx];  out[b,h] = softmax over visible(b) of sm_scale q[b,h].K[b,h/n_rep,s], applied to V; an empty row gives
+ *   zeros.  Slots outside visible(b) may hold anything (NaN included).
+ * `attn` is filled as for kvq_decode_attn with splits = stages = tail_tokens = n_out = 0, no q_chan_scale and no partial
+ * outputs; max_ctx = cols * page_size at most for a paged cache.
+ * `weights` (fp32 [B, Hkv, >= max_ctx] or NULL; contiguous caches without a window only): also
+ *   weights[b,k,s] += sum over the query heads h of kv head k of softmax_h(s) for every s < n_b.
+ * The work is cut into equal runs of token tiles over all rows, one run per resident CTA, so that a ragged batch costs
+ * what its tokens cost; no atomics, results do not change from call to call.  No counterpart in the reference.
+ */
+typedef struct KvqSpanAttnArgs {
+    KvqAttnArgs attn;
+    KvqPageTable pages;
+    int32_t window;              /* last tokens that stay visible, the newest included; 0 = all */
+    int32_t sinks;               /* first tokens that stay visible; only with a window       */
+    float*  weights;
+    int64_t w_stride_b, w_stride_h;                     /* elements                      */
+} KvqSpanAttnArgs;
+
+KVQ_API int kvq_span_attn(const KvqSpanAttnArgs* args, kvq_stream_t stream);
+/* Bytes of attn.workspace this call needs (host query; depends on the current device).  0 = invalid arguments. */
+KVQ_API size_t kvq_span_attn_workspace_bytes(const KvqSpanAttnArgs* args);
+/* 1: these arguments take the tensor-core kernel, 0: the generic one, negative: KVQ_E* (host query). */
+KVQ_API int kvq_span_attn_kernel_kind(const KvqSpanAttnArgs* args);
+
+/*
+ * kvq_quantize_append into pages: token t < new_lens[b] of row b is written at position start_pos[b] + t of the row
+ * (new_lens == NULL: all T tokens).  Same arithmetic, bit for bit.  `append` is filled as for kvq_quantize_append
+ * except write_pos / write_pos_dev / max_slots (0 / NULL / 0), rope_* and outliers (unused: refused).  A token whose
+ * page is not in the table's `cols` or not in [0, num_pages) stores nothing and raises bit 3 of kvq_debug_error_flag.
+ */
+typedef struct KvqPagedAppendArgs {
+    KvqAppendArgs append;
+    KvqPageTable pages;
+    const int32_t* start_pos;    /* int32 [B]                                                */
+    const int32_t* new_lens;     /* int32 [B] or NULL; clamped to [0, T]                     */
+} KvqPagedAppendArgs;
+
+KVQ_API int kvq_paged_append(const KvqPagedAppendArgs* args, kvq_stream_t stream);
+
+/*
+ * Read tokens start_pos[b] + t, t < lens[b], of every row back as fp16 [B, Hkv, T, D]; zeros for t >= lens[b].
+ * value = RN16(code * scale + zero_point), one rounding.
+ */
+typedef struct KvqPagedReadArgs {
+    int32_t format;              /* KVQ_FMT_*                                                */
+    int32_t B, Hkv, T, D;
+    int32_t group_size;
+    KvqPageTable pages;
+    const int32_t* start_pos;    /* int32 [B] or NULL (0)                                    */
+    const int32_t* lens;         /* int32 [B] or NULL (T); clamped to [0, T]                 */
+    KvqCacheSide k, v;
+    void* k_out;                 /* fp16, 16-byte aligned                                    */
+    void* v_out;
+    int64_t out_stride_b, out_stride_h, out_stride_t;   /* elements, multiples of 8; D contiguous */
+} KvqPagedReadArgs;
+
+KVQ_API int kvq_paged_read(const KvqPagedReadArgs* args, kvq_stream_t stream);
+
+/*
+ * Shrink every (batch row, kv head) of a contiguous cache to `budget` tokens.
+ *   n_b = lengths[b] clamped to [0, cap]; the position of slot s is positions[b,h,s] if >= 0, else seen[b] - n_b + s (a
+ *   token appended since the last eviction);
+ *   kept = tokens with position < sinks or >= seen[b] - recent first, then the largest weights; equal weights: the lowest
+ *   slot first; NaN counts as -inf.  Exactly budget tokens.
+ *   Kept tokens in slots < budget stay.  The i-th kept token behind them (slots ascending) moves to the i-th freed slot:
+ *   its row of every buffer, its weight, its position.  Afterwards positions of slots < budget are >= 0, positions of
+ *   slots budget..n_b-1 are -1 and their weights 0; buffer rows behind the budget and all slots >= n_b are left as they were.
+ *   new_lengths[b] = min(n_b, budget) (may alias lengths).  Rows with n_b <= budget are left as they were.
+ * Keys carry their rotary position, so their order in the cache does not matter to kvq_decode_attn.
+ */
+#define KVQ_EVICT_MAX_BUFS 10
+typedef struct KvqEvictBuf {
+    void*   base;                /* [B, Hkv, cap, row]                                       */
+    int64_t stride_b, stride_h, stride_s;               /* BYTES                         */
+    int64_t row_bytes;           /* > 0                                                      */
+} KvqEvictBuf;
+
+typedef struct KvqEvictArgs {
+    int32_t B, Hkv, cap;
+    int32_t budget, sinks, recent;                      /* sinks + recent <= budget      */
+    const int32_t* lengths;      /* int32 [B]                                                */
+    const int32_t* seen;         /* int32 [B]: tokens the row has seen in all                */
+    int32_t* new_lengths;        /* int32 [B]                                                */
+    float*   weights;            /* fp32 [B, Hkv, cap], slots contiguous                     */
+    int64_t  w_stride_b, w_stride_h;                    /* elements                      */
+    int32_t* positions;          /* int32 [B, Hkv, cap], slots contiguous                    */
+    int64_t  p_stride_b, p_stride_h;                    /* elements                      */
+    int32_t  n_bufs;             /* <= KVQ_EVICT_MAX_BUFS                                    */
+    KvqEvictBuf bufs[KVQ_EVICT_MAX_BUFS];
+    void*   workspace;           /* >= kvq_evict_workspace_bytes(...)                        */
+    size_t  workspace_bytes;
+} KvqEvictArgs;
+
+KVQ_API int kvq_evict(const KvqEvictArgs* args, kvq_stream_t stream);
+KVQ_API size_t kvq_evict_workspace_bytes(int32_t B, int32_t Hkv, int32_t cap, int32_t budget);
+
+/*
  * Device-side error flags (synchronises the device): 0 = clean.  Bit 0 (1): a bounded wait on a
  * copy-completion barrier expired inside the tensor-core decode kernel (results of that launch
  * are invalid).  Bit 1 (2): kvq_quantize_append met a device-side position at or beyond
  * max_slots and skipped the stores of that token.  Bit 2 (4): the same for kvq_kivi_append.
+ * Bit 3 (8): a page table entry that was needed lay outside the pool (see KvqPageTable).
  * `reset` != 0 clears them.  Negative = KVQ_E*.  No reference counterpart.
  */
 KVQ_API int kvq_debug_error_flag(int reset);
@@ -438,7 +558,8 @@ KVQ_API int  kvq_last_cuda_error(void);     /* cudaError_t of the last KVQ_ECUDA
 KVQ_API int  kvq_abi_version(void);
 /* sizeof of an argument struct as this library was compiled, for binders that mirror the structs by hand
  * (ctypes, cgo): 0 KvqAppendSide, 1 KvqAppendArgs, 2 KvqCacheSide, 3 KvqAttnArgs, 4 KvqCombineArgs,
- * 5 KvqDequantArgs, 6 KvqKiviArgs, 7 KvqAbsmaxArgs, 8 KvqExchangeArgs, 9 KvqQuantileArgs; 0 for any other id.  No reference counterpart. */
+ * 5 KvqDequantArgs, 6 KvqKiviArgs, 7 KvqAbsmaxArgs, 8 KvqExchangeArgs, 9 KvqQuantileArgs,
+ * 10 KvqPageTable, 11 KvqSpanAttnArgs, 12 KvqPagedAppendArgs, 13 KvqPagedReadArgs, 14 KvqEvictBuf, 15 KvqEvictArgs; 0 for any other id.  No reference counterpart. */
 KVQ_API size_t kvq_struct_size(int which);
 
 #ifdef __cplusplus

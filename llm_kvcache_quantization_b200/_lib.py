@@ -139,6 +139,52 @@ class KvqExchangeArgs(C.Structure):
     ]
 
 
+class KvqPageTable(C.Structure):
+    _fields_ = [
+        ("table", _vp), ("stride_b", _i64), ("cols", _i32), ("page_size", _i32), ("num_pages", _i32),
+    ]
+
+
+class KvqSpanAttnArgs(C.Structure):
+    _fields_ = [
+        ("attn", KvqAttnArgs), ("pages", KvqPageTable), ("window", _i32), ("sinks", _i32),
+        ("weights", _vp), ("w_stride_b", _i64), ("w_stride_h", _i64),
+    ]
+
+
+class KvqPagedAppendArgs(C.Structure):
+    _fields_ = [
+        ("append", KvqAppendArgs), ("pages", KvqPageTable), ("start_pos", _vp), ("new_lens", _vp),
+    ]
+
+
+class KvqPagedReadArgs(C.Structure):
+    _fields_ = [
+        ("format", _i32), ("B", _i32), ("Hkv", _i32), ("T", _i32), ("D", _i32), ("group_size", _i32),
+        ("pages", KvqPageTable), ("start_pos", _vp), ("lens", _vp),
+        ("k", KvqCacheSide), ("v", KvqCacheSide), ("k_out", _vp), ("v_out", _vp),
+        ("out_stride_b", _i64), ("out_stride_h", _i64), ("out_stride_t", _i64),
+    ]
+
+
+EVICT_MAX_BUFS = 10
+
+
+class KvqEvictBuf(C.Structure):
+    _fields_ = [("base", _vp), ("stride_b", _i64), ("stride_h", _i64), ("stride_s", _i64), ("row_bytes", _i64)]
+
+
+class KvqEvictArgs(C.Structure):
+    _fields_ = [
+        ("B", _i32), ("Hkv", _i32), ("cap", _i32), ("budget", _i32), ("sinks", _i32), ("recent", _i32),
+        ("lengths", _vp), ("seen", _vp), ("new_lengths", _vp),
+        ("weights", _vp), ("w_stride_b", _i64), ("w_stride_h", _i64),
+        ("positions", _vp), ("p_stride_b", _i64), ("p_stride_h", _i64),
+        ("n_bufs", _i32), ("bufs", KvqEvictBuf * EVICT_MAX_BUFS),
+        ("workspace", _vp), ("workspace_bytes", C.c_size_t),
+    ]
+
+
 # every symbol include/kvq.h declares: (name, restype, argtypes)
 EXPORTS = (
     ("kvq_quantize_append", C.c_int, (C.POINTER(KvqAppendArgs), _vp)),
@@ -154,6 +200,13 @@ EXPORTS = (
     ("kvq_kivi_dequantize", C.c_int, (C.POINTER(KvqKiviArgs), _vp)),
     ("kvq_group_absmax", C.c_int, (C.POINTER(KvqAbsmaxArgs), _vp)),
     ("kvq_dequantize", C.c_int, (C.POINTER(KvqDequantArgs), _vp)),
+    ("kvq_span_attn", C.c_int, (C.POINTER(KvqSpanAttnArgs), _vp)),
+    ("kvq_span_attn_workspace_bytes", C.c_size_t, (C.POINTER(KvqSpanAttnArgs),)),
+    ("kvq_span_attn_kernel_kind", C.c_int, (C.POINTER(KvqSpanAttnArgs),)),
+    ("kvq_paged_append", C.c_int, (C.POINTER(KvqPagedAppendArgs), _vp)),
+    ("kvq_paged_read", C.c_int, (C.POINTER(KvqPagedReadArgs), _vp)),
+    ("kvq_evict", C.c_int, (C.POINTER(KvqEvictArgs), _vp)),
+    ("kvq_evict_workspace_bytes", C.c_size_t, (_i32, _i32, _i32, _i32)),
     ("kvq_debug_error_flag", C.c_int, (C.c_int,)),
     ("kvq_selftest_division", C.c_int, (C.c_int, C.c_uint32, C.POINTER(C.c_uint64), C.POINTER(C.c_uint64))),
     ("kvq_decode_kernel_kind", C.c_int, (C.POINTER(KvqAttnArgs),)),
@@ -166,7 +219,8 @@ EXPORTS = (
 ABI_VERSION = 5
 # ids of kvq_struct_size, in the order of include/kvq.h
 STRUCTS = (KvqAppendSide, KvqAppendArgs, KvqCacheSide, KvqAttnArgs, KvqCombineArgs, KvqDequantArgs, KvqKiviArgs,
-           KvqAbsmaxArgs, KvqExchangeArgs, KvqQuantileArgs)
+           KvqAbsmaxArgs, KvqExchangeArgs, KvqQuantileArgs, KvqPageTable, KvqSpanAttnArgs, KvqPagedAppendArgs,
+           KvqPagedReadArgs, KvqEvictBuf, KvqEvictArgs)
 
 _LIB = None
 

@@ -67,6 +67,11 @@ class _CacheBase:
         self._dev_positions = None
         self._layer_capacity: List[int] = [0] * num_layers
         self._seq_len = 0
+        self._window: Optional[Tuple[int, int]] = None       # (window, sinks) of set_attention_window
+        self._evict: Optional[Tuple[int, int, int]] = None   # (budget, sinks, recent) of enable_eviction
+        self._evict_state: List[Optional[Dict[str, Tensor]]] = [None] * num_layers
+        self._layer_seen: List[int] = [0] * num_layers       # with eviction: tokens appended, evicted ones included
+        self._row_ints: Dict[str, Tuple[Tuple[int, int], Tensor]] = {}
         self.decode_stats: Dict[str, object] = _new_stats()
 
     # ---- decode statistics (key names are read by the reference's callers/tests)
@@ -173,6 +178,7 @@ class _CacheBase:
     def _finish_append(self, layer_id: int, target_len: int) -> None:
         if self._dev_positions is not None:
             return                                   # lengths live on the device; advance_host_lengths() follows
+        self._layer_seen[layer_id] += target_len - self._layer_seq_lens[layer_id]
         self._layer_seq_lens[layer_id] = target_len
         if layer_id == 0:
             self._seq_len = target_len
@@ -181,6 +187,8 @@ class _CacheBase:
     # single-token appends write at `*pos` (int32 device scalar), fused_decode attends over `ctx` (int32 [B]
     # device tensor) inside views of the first `capacity` slots, and nothing here touches host-side lengths.
     def use_device_positions(self, pos: Tensor, ctx: Tensor, capacity: int) -> None:
+        if self._evict is not None:
+            raise ValueError("eviction changes the lengths on the host: it does not go with device-side positions")
         if pos.dtype != torch.int32 or ctx.dtype != torch.int32 or not pos.is_cuda or not ctx.is_cuda:
             raise ValueError("pos / ctx must be int32 CUDA tensors")
         for l in range(self.num_layers):
@@ -196,6 +204,94 @@ class _CacheBase:
         for l in range(self.num_layers):
             self._layer_seq_lens[l] += tokens
         self._seq_len = self._layer_seq_lens[0]
+
+    # ---- bounded attention and bounded memory
+    def set_attention_window(self, window: Optional[int], sinks: int = 0) -> None:
+        """From now on `fused_decode` attends only the last `window` cached tokens and the first `sinks` (None: all).  The
+        cache keeps every token."""
+        if window is None:
+            if sinks:
+                raise ValueError("sinks go with a window")
+            self._window = None
+            return
+        if window < 1 or sinks < 0:
+            raise ValueError(f"window must be >= 1 and sinks >= 0, got {window}, {sinks}")
+        if self._evict is not None:
+            raise ValueError("a cache with eviction holds its tokens out of order: it takes no attention window")
+        self._check_span_format("an attention window")
+        self._window = (int(window), int(sinks))
+
+    def enable_eviction(self, budget: int, sinks: int = 4, recent: int = 32) -> None:
+        """Bound every layer to `budget` tokens per kv head.  `fused_decode` then also accumulates the attention weights of
+        the cached tokens and, when the layer holds more than the budget, evicts: the first `sinks` and the last `recent`
+        tokens of the sequence stay, then those with the largest accumulated weight (`evict_tokens`).  Weights count from
+        here on, so a prompt is ranked by the first decode step.  Positions of the evicted tokens are not reused:
+        `get_tokens_seen()` is the position of the next token, `get_seq_len()` the number of cached ones."""
+        if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
+            raise ValueError(f"need budget >= 1 and 0 <= sinks + recent <= budget, got {budget}, {sinks}, {recent}")
+        if self._window is not None:
+            raise ValueError("a cache with an attention window takes no eviction")
+        if self._dev_positions is not None:
+            raise ValueError("eviction changes the lengths on the host: it does not go with device-side positions")
+        if self._evict is not None:
+            raise ValueError("eviction is already enabled")
+        self._check_span_format("eviction")
+        self._layer_seen = list(self._layer_seq_lens)        # nothing was evicted before
+        self._evict = (int(budget), int(sinks), int(recent))
+
+    def _check_span_format(self, what: str) -> None:
+        """Raise for the formats and implementations that have no span kernel."""
+        if getattr(self, "decode_attn_impl", "triton_fused") != "triton_fused":
+            raise ValueError(f"{what} needs the fused decode kernels (decode_attn_impl='triton_fused'), "
+                             f"got {self.decode_attn_impl!r}")
+
+    def get_tokens_seen(self) -> int:
+        """Tokens appended to layer 0 since `clear()`, evicted ones included: the position of the next token."""
+        return self._layer_seen[0] if self._evict is not None else self._seq_len
+
+    def _row_int(self, name: str, value: int, batch: int, device) -> Tensor:
+        """int32 [batch] device tensor of one value; the layers of a step share it."""
+        key, t = self._row_ints.get(name, (None, None))
+        if key != (value, batch) or t.device != device:
+            t = torch.full((batch,), value, dtype=torch.int32, device=device)
+            self._row_ints[name] = ((value, batch), t)
+        return t
+
+    def _eviction_buffers(self, layer_id: int) -> Dict[str, Tensor]:
+        """Accumulated weights and positions of one layer, as long as its buffers."""
+        k = self._bufs[layer_id]["k"]
+        st = self._evict_state[layer_id]
+        if st is None or st["w"].shape != k.shape[:3]:
+            new = {"w": torch.zeros(k.shape[:3], dtype=torch.float32, device=k.device),
+                   "p": torch.full(k.shape[:3], -1, dtype=torch.int32, device=k.device)}
+            if st is not None:                               # the layer's buffers grew
+                for name in new:
+                    new[name][:, :, :st[name].shape[2]] = st[name]
+            self._evict_state[layer_id] = st = new
+        return st
+
+    def _span_decode(self, layer_id: int, q: Tensor, parts, sm_scale: float, inv_tau, out) -> Tensor:
+        """fused_decode under a window or with eviction; `parts` = (k, v, k_scale, v_scale, k_zp, v_zp) views."""
+        k, v, ks, vs, kz, vz = parts
+        kw = dict(k_zp=kz, v_zp=vz, inv_tau=inv_tau, out=out)
+        if self._window is not None:
+            ctx = None if self._dev_positions is None else self._dev_positions[1]
+            return ops.span_attn(q, k, v, ks, vs, ctx, sm_scale, window=self._window[0], sinks=self._window[1], **kw)
+        budget, sinks, recent = self._evict
+        st = self._eviction_buffers(layer_id)
+        res = ops.span_attn(q, k, v, ks, vs, None, sm_scale, weights=st["w"], **kw)
+        n = self._layer_seq_lens[layer_id]
+        if n > budget:
+            bufs = self._bufs[layer_id]
+            B = k.shape[0]
+            # slots behind the cached tokens are not looked at: views of the first n keep the scratch memory small
+            ops.evict(st["w"][:, :, :n], st["p"][:, :, :n], self._row_int("n", n, B, k.device),
+                      self._row_int("seen", self._layer_seen[layer_id], B, k.device), budget,
+                      [t[:, :, :n] for t in bufs.values()], sinks=sinks, recent=recent)
+            self._layer_seq_lens[layer_id] = budget
+            if layer_id == 0:
+                self._seq_len = budget
+        return res
 
     def _write_slot(self, layer_id: int, batch: int, heads: int, head_dim: int, tokens: int):
         """(first slot to write - an int, or the device scalar -, host length before the append)."""
@@ -239,12 +335,19 @@ class _CacheBase:
         """Reset lengths, keep the buffers."""
         self._layer_seq_lens = [0] * self.num_layers
         self._seq_len = 0
+        self._forget_evictions()
+
+    def _forget_evictions(self) -> None:
+        self._layer_seen = [0] * self.num_layers
+        self._evict_state = [None] * self.num_layers
+        self._row_ints.clear()
 
     def release(self) -> None:
         self._bufs = [None] * self.num_layers
         self._layer_seq_lens = [0] * self.num_layers
         self._layer_capacity = [0] * self.num_layers
         self._seq_len = 0
+        self._forget_evictions()
 
     def get_memory_mb(self) -> float:
         total = 0
@@ -313,6 +416,9 @@ class FP16KVCache(_CacheBase):
         original = q.dtype
         if original != torch.float16:
             q = q.to(torch.float16)
+        if self._window is not None or self._evict is not None:
+            res = self._span_decode(layer_id, q, (k, v, None, None, None, None), float(sm_scale), inv_tau, out)
+            return res if original == torch.float16 else res.to(original)
         ctx = None if self._dev_positions is None else self._dev_positions[1]
         res = ops.decode_attn(FMT_FP16, q, k, v, None, None, ctx, float(sm_scale), head_dim=q.shape[-1],
                               inv_tau=None if inv_tau is None else inv_tau.float(), out=out)
@@ -494,6 +600,11 @@ class _QuantCache(_CacheBase):
                     f"capacity (threshold={_CLIP_WARN_THRESHOLD:.0%}). Consider re-calibrating or enabling "
                     "adaptive_static_scales.", RuntimeWarning)
 
+    def _check_span_format(self, what: str) -> None:
+        super()._check_span_format(what)
+        if self.outlier_idx is not None:
+            raise ValueError(f"{what} is not available for a cache with outlier side buffers")
+
     def get_fp32_scales(self, layer_id: int) -> Tuple[Tensor, Tensor]:
         if not self.keep_fp32_scales:
             raise ValueError("construct the cache with keep_fp32_scales=True to keep fp32 scale copies")
@@ -519,6 +630,10 @@ class _QuantCache(_CacheBase):
         original = q.dtype
         if original != torch.float16:
             q = q.to(torch.float16)
+        if self._window is not None or self._evict is not None:
+            res = self._span_decode(layer_id, q, (t["k"], t["v"], t["ks"], t["vs"], t.get("kz"), t.get("vz")),
+                                    float(sm_scale), inv_tau, out)
+            return res if original == torch.float16 else res.to(original)
         extra = {}
         if self.asymmetric:
             extra.update(k_zp=t["kz"], v_zp=t["vz"])

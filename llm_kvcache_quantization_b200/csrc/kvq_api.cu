@@ -61,6 +61,12 @@ extern "C" size_t kvq_struct_size(int which) {
         case 7: return sizeof(KvqAbsmaxArgs);
         case 8: return sizeof(KvqExchangeArgs);
         case 9: return sizeof(KvqQuantileArgs);
+        case 10: return sizeof(KvqPageTable);
+        case 11: return sizeof(KvqSpanAttnArgs);
+        case 12: return sizeof(KvqPagedAppendArgs);
+        case 13: return sizeof(KvqPagedReadArgs);
+        case 14: return sizeof(KvqEvictBuf);
+        case 15: return sizeof(KvqEvictArgs);
         default: return 0;
     }
 }

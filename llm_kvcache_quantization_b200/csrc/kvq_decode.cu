@@ -996,8 +996,9 @@ extern "C" int kvq_debug_error_flag(int reset) {
         if (cudaMemcpyToSymbol(kvq::g_kvq_error_flag, &z, sizeof(int)) != cudaSuccess) return KVQ_ECUDA;
     }
     const int qf = kvq::quantize_error_flag(reset), kf = kvq::kivi_error_flag(reset);
-    if (qf < 0 || kf < 0) return KVQ_ECUDA;
-    return (v ? 1 : 0) | (qf ? 2 : 0) | (kf ? 4 : 0);
+    const int sf = kvq::span_error_flag(reset), pf = kvq::page_error_flag(reset), rf = kvq::paged_read_error_flag(reset);
+    if (qf < 0 || kf < 0 || sf < 0 || pf < 0 || rf < 0) return KVQ_ECUDA;
+    return ((v || (sf & 1)) ? 1 : 0) | (qf ? 2 : 0) | (kf ? 4 : 0) | (((sf & 2) || pf || rf) ? 8 : 0);
 }
 
 extern "C" int kvq_lse_combine(const KvqCombineArgs* args, kvq_stream_t stream) {

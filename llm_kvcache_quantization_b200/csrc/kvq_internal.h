@@ -24,6 +24,9 @@ int device_sm_count();
 // cleared; negative = KVQ_ECUDA.  kvq_debug_error_flag combines them.
 int quantize_error_flag(int reset);
 int kivi_error_flag(int reset);
+int span_error_flag(int reset);     // the three page lookups: attention, append, read-back
+int page_error_flag(int reset);
+int paged_read_error_flag(int reset);
 
 // Launch with programmatic dependent launch: the grid may start while the previous kernel in the
 // stream is still running; the kernel itself calls pdl_wait() before it touches anything that

@@ -42,7 +42,28 @@ struct QuantParams {
     int G;
     int nsides;   // 2, or 1 when the V side is absent (v.src == NULL)
     long long q_items;   // B * Hq * T * G work items that rotate the query (0 = none)
+    // PAGED instantiations: the destination buffers are page pools
+    KvqPageTable pg;
+    const int32_t* start_pos;
+    const int32_t* new_lens;
 };
+
+__device__ int g_page_error_flag = 0;       // 1: a token's page lay outside the table or the pool
+
+// Pool page and row of position `pos` of batch row b; false (and the flag) when there is no such page.
+__device__ __forceinline__ bool page_of(const KvqPageTable& pg, int b, long long pos, long long& page, long long& row) {
+    const int blk = pos >= 0 && pos <= 0x7fffffffLL ? (int)pos / pg.page_size : -1;
+    int id = -1;
+    if (blk >= 0 && blk < pg.cols) id = pg.table[b * pg.stride_b + blk];
+    if (id < 0 || id >= pg.num_pages) {
+        g_page_error_flag = 1;
+        page = row = 0;
+        return false;
+    }
+    page = id;
+    row = (int)pos - blk * pg.page_size;
+    return true;
+}
 
 __device__ __forceinline__ float h2f(__half h) { return __half2float(h); }
 
@@ -192,7 +213,9 @@ __global__ void selftest_div_full_kernel(uint32_t stride, uint32_t first, uint32
 //           CH * LPG channels: LPG adjacent lanes (1, 2 or 4) share it and combine their statistics with
 //           warp shuffles, so groups of 64 and 128 channels keep the 32-channel register footprint.
 //   CH == 0: any group size, one thread per group, element-wise loads.
-template <int FMT, int POLICY, int CH, int LPG>
+//   PAGED: positions start_pos[b] + t of the row, looked up in the page table (kvq_paged_append); tokens from new_lens[b]
+//           on store nothing.
+template <int FMT, int POLICY, int CH, int LPG, bool PAGED>
 __global__ void __launch_bounds__(128) quantize_append_kernel(const QuantParams p) {
     pdl_launch_dependents();      // the decode kernel that follows may start its prologue now
     pdl_wait();                   // launched early itself: the kernel before it may still produce the new tokens
@@ -232,14 +255,21 @@ __global__ void __launch_bounds__(128) quantize_append_kernel(const QuantParams 
     const int t = (int)(r % a.T); r /= a.T;
     const int h = (int)(r % a.Hkv);
     const int b = (int)(r / a.Hkv);
-    long long pos = a.write_pos_dev ? (long long)(*a.write_pos_dev) : a.write_pos;
-    pos += t;
-    // a slot beyond the destination buffers (a graph replayed once too often, a stale device counter): nothing of
-    // this token is stored, the flag is raised, and the lane keeps running so that group shuffles stay complete
-    const bool in_range = a.max_slots <= 0 || (pos >= 0 && pos < a.max_slots);
-    if (!in_range) {
-        g_quantize_error_flag = 1;
+    long long pos, major = b;                               // slot, and batch row or page
+    bool in_range;
+    if constexpr (PAGED) {
+        in_range = !p.new_lens || t < p.new_lens[b];
         pos = 0;
+        if (in_range) in_range = page_of(p.pg, b, (long long)p.start_pos[b] + t, major, pos);
+    } else {
+        pos = (a.write_pos_dev ? (long long)(*a.write_pos_dev) : a.write_pos) + t;
+        // a slot beyond the destination buffers (a graph replayed once too often, a stale device counter): nothing of
+        // this token is stored, the flag is raised, and the lane keeps running so that group shuffles stay complete
+        in_range = a.max_slots <= 0 || (pos >= 0 && pos < a.max_slots);
+        if (!in_range) {
+            g_quantize_error_flag = 1;
+            pos = 0;
+        }
     }
 
     const __half* src = (const __half*)sd.src + b * sd.src_stride_b + h * sd.src_stride_h +
@@ -248,7 +278,7 @@ __global__ void __launch_bounds__(128) quantize_append_kernel(const QuantParams 
     const bool rope = a.rope_cos != nullptr && sidx == 0;
     const __half* rcos = rope ? (const __half*)a.rope_cos + b * a.rope_stride_b + t * a.rope_stride_t : nullptr;
     const __half* rsin = rope ? (const __half*)a.rope_sin + b * a.rope_stride_b + t * a.rope_stride_t : nullptr;
-    char* pay = (char*)sd.payload + b * sd.pay_stride_b + h * sd.pay_stride_h + pos * sd.pay_stride_s;
+    char* pay = (char*)sd.payload + major * sd.pay_stride_b + h * sd.pay_stride_h + pos * sd.pay_stride_s;
 
     if (FMT == KVQ_FMT_FP16) {
         __half* dst = (__half*)pay + cb;
@@ -348,7 +378,7 @@ __global__ void __launch_bounds__(128) quantize_append_kernel(const QuantParams 
         return amax;
     };
 
-    const long long sc_off = b * sd.sc_stride_b + h * sd.sc_stride_h + pos * sd.sc_stride_s + g;
+    const long long sc_off = major * sd.sc_stride_b + h * sd.sc_stride_h + pos * sd.sc_stride_s + g;
     float s32 = 1.0f, zp32 = 0.0f;   // scale used for the division (fp32 value)
 
     if (POLICY == KVQ_SCALE_STATIC) {
@@ -494,7 +524,7 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
     return r;
 }
 
-template <int FMT, int POLICY, int CH, int LPG, int U>
+template <int FMT, int POLICY, int CH, int LPG, int U, bool PAGED>
 __global__ void __launch_bounds__(256) quantize_bulk_kernel(const QuantParams p) {
     pdl_launch_dependents();
     pdl_wait();
@@ -509,11 +539,12 @@ __global__ void __launch_bounds__(256) quantize_bulk_kernel(const QuantParams p)
     const int b = blockIdx.z - (sidx ? a.B : 0);
     const KvqAppendSide sd = sidx ? a.v : a.k;             // by value: the fields used below are selected once
     const int g = c / LPG, cb = c * CH;
-    const int flags = a.flags, n_out = a.n_out, T = a.T;
-    const long long pos0 = a.write_pos_dev ? (long long)(*a.write_pos_dev) : a.write_pos;
+    const int flags = a.flags, n_out = a.n_out;
+    const int T = PAGED && p.new_lens ? max(0, min(a.T, p.new_lens[b])) : a.T;
+    const long long pos0 = PAGED ? (long long)p.start_pos[b] : a.write_pos_dev ? (long long)(*a.write_pos_dev) : a.write_pos;
     // tokens [t_lo, t_hi) have a slot inside the destination buffers (slot = pos0 + t); the others store nothing
-    const int t_lo = (a.max_slots > 0 && pos0 < 0) ? (int)min(-pos0, (long long)T) : 0;
-    const int t_hi = a.max_slots > 0 ? (int)max(0ll, min((long long)T, a.max_slots - pos0)) : T;
+    const int t_lo = (!PAGED && a.max_slots > 0 && pos0 < 0) ? (int)min(-pos0, (long long)T) : 0;
+    const int t_hi = (!PAGED && a.max_slots > 0) ? (int)max(0ll, min((long long)T, a.max_slots - pos0)) : T;
     if (t_lo > 0 || t_hi < T) g_quantize_error_flag = 1;
     const int t_base = blockIdx.x * (rows * U) + rloc;
     // everything of token t_base; pass u is u * rows tokens further
@@ -548,8 +579,10 @@ __global__ void __launch_bounds__(256) quantize_bulk_kernel(const QuantParams p)
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int t = t_base + u * rows;
-        const bool in_range = t >= t_lo && t < t_hi;       // other rows compute (on zeros past T) and store nothing
+        bool in_range = t >= t_lo && t < t_hi;             // other rows compute (on zeros past T) and store nothing
         uint32_t* w = raw[u];
+        long long page = 0, prow = 0;
+        if (PAGED && in_range) in_range = page_of(p.pg, b, pos0 + t, page, prow);
         if (oidx) {
             __half* side = sd.side ? (__half*)sd.side + b * sd.side_stride_b + h * sd.side_stride_h + (pos0 + t) * sd.side_stride_s : nullptr;
             for (int j = 0; j < n_out; ++j) {
@@ -644,7 +677,7 @@ __global__ void __launch_bounds__(256) quantize_bulk_kernel(const QuantParams p)
         const __half s16 = __float2half_rn(s32);
         if (FMT == KVQ_FMT_INT8 && POLICY != KVQ_SCALE_ASYM_MINMAX) s32 = h2f(s16);
         if (in_range && (c % LPG) == 0) {
-            const long long sc_off = sc_t + u * sc_step;
+            const long long sc_off = PAGED ? page * sd.sc_stride_b + h * sd.sc_stride_h + prow * sd.sc_stride_s + g : sc_t + u * sc_step;
             ((__half*)sd.scale)[sc_off] = s16;
             if (sd.scale_f32) sd.scale_f32[sc_off] = s32;
             if (POLICY == KVQ_SCALE_ASYM_MINMAX) ((__half*)sd.zp)[sc_off] = __float2half_rn(zp32);
@@ -654,7 +687,7 @@ __global__ void __launch_bounds__(256) quantize_bulk_kernel(const QuantParams p)
         constexpr float lo_b = (POLICY == KVQ_SCALE_ASYM_MINMAX) ? (FMT == KVQ_FMT_INT8 ? -128.f : -8.f) : (FMT == KVQ_FMT_INT8 ? -127.f : -7.f);
         constexpr float hi_b = (FMT == KVQ_FMT_INT8) ? 127.f : 7.f;
         if (!in_range) continue;
-        char* pay = pay_t + u * pay_step;
+        char* pay = PAGED ? (char*)sd.payload + page * sd.pay_stride_b + h * sd.pay_stride_h + prow * sd.pay_stride_s : pay_t + u * pay_step;
         constexpr float kMagic = 12582912.0f;              // 1.5 * 2^23: ulp 1
         // the codes of the chunk; IEEE = true divides with __fdiv_rn (chunks with a value that is not finite)
         auto emit = [&](auto ieee) {
@@ -725,14 +758,14 @@ __global__ void __launch_bounds__(256) quantize_bulk_kernel(const QuantParams p)
     }
 }
 
-template <int FMT, int POLICY, int CH, int LPG>
+template <int FMT, int POLICY, int CH, int LPG, bool PAGED>
 static int launch_bulk(const QuantParams& p, cudaStream_t st) {
     constexpr int U = 4;
     const int cpr = p.a.D / CH, rows = 256 / cpr;
     const long long tiles = ((long long)p.a.T + rows * U - 1) / (rows * U);
     const long long gz = (long long)p.nsides * p.a.B;
     if (tiles > 0x7fffffffLL || p.a.Hkv > 65535 || gz > 65535) return KVQ_EUNSUPPORTED;
-    return launch_pdl(quantize_bulk_kernel<FMT, POLICY, CH, LPG, U>, dim3((unsigned)tiles, (unsigned)p.a.Hkv, (unsigned)gz), dim3(256),
+    return launch_pdl(quantize_bulk_kernel<FMT, POLICY, CH, LPG, U, PAGED>, dim3((unsigned)tiles, (unsigned)p.a.Hkv, (unsigned)gz), dim3(256),
                       0, st, p);
 }
 
@@ -762,7 +795,7 @@ static bool side_vec_ok(const KvqAppendSide& s) {
                       (s.src_stride_t & 7) == 0);
 }
 
-template <int FMT, int POLICY, int CH, int LPG>
+template <int FMT, int POLICY, int CH, int LPG, bool PAGED>
 static int launch_gs(const QuantParams& p, cudaStream_t st) {
     const int cpr = CH ? p.a.D / CH : p.G;
     const long long per_row_set = (long long)p.a.B * p.a.T * cpr;
@@ -773,10 +806,10 @@ static int launch_gs(const QuantParams& p, cudaStream_t st) {
     if (grid > 0x7fffffffLL) return KVQ_EINVAL;
     QuantParams q = p;
     q.q_items = p.q_items ? per_row_set * p.a.Hq : 0;
-    return launch_pdl(quantize_append_kernel<FMT, POLICY, CH, LPG>, dim3((unsigned)grid), dim3(block), 0, st, q);
+    return launch_pdl(quantize_append_kernel<FMT, POLICY, CH, LPG, PAGED>, dim3((unsigned)grid), dim3(block), 0, st, q);
 }
 
-template <int FMT, int POLICY>
+template <int FMT, int POLICY, bool PAGED = false>
 static int launch(const QuantParams& p, cudaStream_t st) {
     const KvqAppendArgs& a = p.a;
     const int gs = a.group_size;
@@ -784,10 +817,10 @@ static int launch(const QuantParams& p, cudaStream_t st) {
     const bool dyn_sort = POLICY == KVQ_SCALE_DYNAMIC_PCT && a.quantile < 1.0f && !top2_applies(gs, a.quantile);
     if constexpr (FMT != KVQ_FMT_FP16) if (bulk_ok<FMT, POLICY>(p)) {
         int rc = KVQ_EUNSUPPORTED;
-        if (gs == 16) rc = launch_bulk<FMT, POLICY, 8, 2>(p, st);
-        if (gs == 32) rc = launch_bulk<FMT, POLICY, 16, 2>(p, st);
-        if (gs == 64) rc = launch_bulk<FMT, POLICY, 16, 4>(p, st);
-        if (gs == 128) rc = launch_bulk<FMT, POLICY, 16, 8>(p, st);
+        if (gs == 16) rc = launch_bulk<FMT, POLICY, 8, 2, PAGED>(p, st);
+        if (gs == 32) rc = launch_bulk<FMT, POLICY, 16, 2, PAGED>(p, st);
+        if (gs == 64) rc = launch_bulk<FMT, POLICY, 16, 4, PAGED>(p, st);
+        if (gs == 128) rc = launch_bulk<FMT, POLICY, 16, 8, PAGED>(p, st);
         if (rc != KVQ_EUNSUPPORTED) return rc;
     }
     const bool rope = a.rope_cos != nullptr;
@@ -795,17 +828,17 @@ static int launch(const QuantParams& p, cudaStream_t st) {
                                        (a.rope_stride_b & 7) == 0 && (a.rope_stride_t & 7) == 0);
     if (!dyn_sort && side_vec_ok(a.k) && side_vec_ok(a.v) && rope_vec_ok) {
         // register-resident chunks of 32 (or 16) channels; rotary partners are whole chunks
-        if (FMT == KVQ_FMT_FP16 && a.D % 32 == 0) return launch_gs<FMT, POLICY, 32, 1>(p, st);   // a plain copy: any chunking
+        if (FMT == KVQ_FMT_FP16 && a.D % 32 == 0) return launch_gs<FMT, POLICY, 32, 1, PAGED>(p, st);   // a plain copy: any chunking
         // a handful of rows (one decode token): spread each group of 32 over two lanes - the per-element division
         // chain of a thread halves, and the launch is a latency chain, not a throughput kernel
         const long long groups = (long long)a.B * a.Hkv * a.T * (a.D / (gs > 0 ? gs : 1)) * p.nsides;
-        if (gs == 32 && FMT != KVQ_FMT_FP16 && groups <= 4096) return launch_gs<FMT, POLICY, 16, 2>(p, st);
-        if (gs == 32) return launch_gs<FMT, POLICY, 32, 1>(p, st);
-        if (gs == 64) return launch_gs<FMT, POLICY, 32, 2>(p, st);
-        if (gs == 128) return launch_gs<FMT, POLICY, 32, 4>(p, st);
-        if (gs == 16) return launch_gs<FMT, POLICY, 16, 1>(p, st);
+        if (gs == 32 && FMT != KVQ_FMT_FP16 && groups <= 4096) return launch_gs<FMT, POLICY, 16, 2, PAGED>(p, st);
+        if (gs == 32) return launch_gs<FMT, POLICY, 32, 1, PAGED>(p, st);
+        if (gs == 64) return launch_gs<FMT, POLICY, 32, 2, PAGED>(p, st);
+        if (gs == 128) return launch_gs<FMT, POLICY, 32, 4, PAGED>(p, st);
+        if (gs == 16) return launch_gs<FMT, POLICY, 16, 1, PAGED>(p, st);
     }
-    return launch_gs<FMT, POLICY, 0, 1>(p, st);
+    return launch_gs<FMT, POLICY, 0, 1, PAGED>(p, st);
 }
 
 static bool side_ok(const KvqAppendSide& s, const KvqAppendArgs& a) {
@@ -827,6 +860,16 @@ int quantize_error_flag(int reset) {
     if (reset && v) {
         const int z = 0;
         if (cudaMemcpyToSymbol(g_quantize_error_flag, &z, sizeof(int)) != cudaSuccess) return KVQ_ECUDA;
+    }
+    return v;
+}
+
+int page_error_flag(int reset) {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_page_error_flag, sizeof(int)) != cudaSuccess) return KVQ_ECUDA;
+    if (reset && v) {
+        const int z = 0;
+        if (cudaMemcpyToSymbol(g_page_error_flag, &z, sizeof(int)) != cudaSuccess) return KVQ_ECUDA;
     }
     return v;
 }
@@ -883,7 +926,7 @@ extern "C" int kvq_quantize_append(const KvqAppendArgs* args, kvq_stream_t strea
     if (a.n_out > 0 && a.policy == KVQ_SCALE_ASYM_MINMAX) return KVQ_EUNSUPPORTED;
     if (a.write_pos < 0 || a.max_slots < 0) return KVQ_EINVAL;
     if (a.max_slots > 0 && !a.write_pos_dev && a.write_pos + a.T > a.max_slots) return KVQ_ELIMIT;
-    QuantParams p;
+    QuantParams p = {};
     p.a = a;
     p.a.group_size = gs;
     p.G = a.D / gs;
@@ -900,6 +943,47 @@ extern "C" int kvq_quantize_append(const KvqAppendArgs* args, kvq_stream_t strea
     cudaStream_t st = (cudaStream_t)stream;
 #define KVQ_DISPATCH(F, P) if (a.format == F && a.policy == P) return launch<F, P>(p, st);
     if (a.format == KVQ_FMT_FP16) return launch<KVQ_FMT_FP16, KVQ_SCALE_STATIC>(p, st);
+    KVQ_DISPATCH(KVQ_FMT_INT8, KVQ_SCALE_STATIC)
+    KVQ_DISPATCH(KVQ_FMT_INT8, KVQ_SCALE_DYNAMIC_PCT)
+    KVQ_DISPATCH(KVQ_FMT_INT8, KVQ_SCALE_ASYM_MINMAX)
+    KVQ_DISPATCH(KVQ_FMT_INT4, KVQ_SCALE_STATIC)
+    KVQ_DISPATCH(KVQ_FMT_INT4, KVQ_SCALE_DYNAMIC_PCT)
+    KVQ_DISPATCH(KVQ_FMT_INT4, KVQ_SCALE_ASYM_MINMAX)
+#undef KVQ_DISPATCH
+    return KVQ_EUNSUPPORTED;
+}
+
+extern "C" int kvq_paged_append(const KvqPagedAppendArgs* args, kvq_stream_t stream) {
+    using namespace kvq;
+    if (!args) return KVQ_EINVAL;
+    const KvqAppendArgs& a = args->append;
+    if (a.B < 0 || a.Hkv <= 0 || a.T < 0 || a.D <= 0) return KVQ_EINVAL;
+    if (a.write_pos || a.write_pos_dev || a.max_slots) return KVQ_EINVAL;
+    if (a.rope_cos || a.rope_sin || a.q_src || a.n_out) return KVQ_EUNSUPPORTED;
+    if (a.format != KVQ_FMT_FP16 && a.format != KVQ_FMT_INT8 && a.format != KVQ_FMT_INT4) return KVQ_EINVAL;
+    if (a.policy < 0 || a.policy > 2) return KVQ_EINVAL;
+    int gs = a.group_size == -1 || a.format == KVQ_FMT_FP16 ? a.D : a.group_size;
+    if (gs <= 0 || a.D % gs != 0 || gs % 8 != 0 || gs > kMaxGroup) return KVQ_EINVAL;
+    if (a.B == 0 || a.T == 0) return KVQ_OK;
+    const KvqPageTable& pg = args->pages;
+    if (!pg.table || !args->start_pos || pg.page_size <= 0 || pg.cols <= 0 || pg.num_pages <= 0) return KVQ_EINVAL;
+    QuantParams p = {};
+    p.a = a;
+    p.a.group_size = gs;
+    p.G = a.D / gs;
+    p.nsides = a.v.src ? 2 : 1;
+    p.pg = pg;
+    p.start_pos = args->start_pos;
+    p.new_lens = args->new_lens;
+    if (!side_ok(a.k, p.a) || (p.nsides == 2 && !side_ok(a.v, p.a))) return KVQ_EINVAL;
+    for (int i = 0; i < p.nsides; ++i) {                   // what the attention kernels ask of a pool
+        const KvqAppendSide& sd = i ? a.v : a.k;
+        if (((uintptr_t)sd.payload | (uintptr_t)sd.pay_stride_b | (uintptr_t)sd.pay_stride_h | (uintptr_t)sd.pay_stride_s) & 15)
+            return KVQ_EINVAL;
+    }
+    cudaStream_t st = (cudaStream_t)stream;
+    if (a.format == KVQ_FMT_FP16) return launch<KVQ_FMT_FP16, KVQ_SCALE_STATIC, true>(p, st);
+#define KVQ_DISPATCH(F, P) if (a.format == F && a.policy == P) return launch<F, P, true>(p, st);
     KVQ_DISPATCH(KVQ_FMT_INT8, KVQ_SCALE_STATIC)
     KVQ_DISPATCH(KVQ_FMT_INT8, KVQ_SCALE_DYNAMIC_PCT)
     KVQ_DISPATCH(KVQ_FMT_INT8, KVQ_SCALE_ASYM_MINMAX)

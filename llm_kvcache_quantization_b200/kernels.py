@@ -250,3 +250,67 @@ def decode_attn_fp16(q, k_cache, v_cache, context_lens, sm_scale: Optional[float
         raise ValueError("GQA head mismatch")
     return _run(FMT_FP16, q, k_cache, v_cache, None, None, context_lens, sm_scale, q.shape[-1],
                 debug_stats, layer_idx, None, inv_tau=inv_tau)
+
+
+# --------------------------------------------------------------------------- bounded and paged caches
+def _span(q, *args, out=None, **kw):
+    """ops.span_attn in q's dtype, as the wrappers above."""
+    if q.dtype == torch.float16:
+        return ops.span_attn(q, *args, out=out, **kw)
+    if out is not None:
+        raise ValueError(f"out is only taken together with an fp16 query, got q {q.dtype}")
+    return ops.span_attn(q.to(torch.float16), *args, **kw).to(q.dtype)
+
+
+def decode_attn_paged(q, k_pages, v_pages, k_scale, v_scale, block_table, context_lens, sm_scale: Optional[float] = None, *,
+                      window: Optional[int] = None, sinks: int = 0, max_ctx: Optional[int] = None,
+                      k_zp=None, v_zp=None, inv_tau: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None):
+    """Attention of one new token per row over a paged cache: q [B,Hq,D]; k_pages / v_pages
+    [num_pages,Hkv,page_size,D] fp16 or int8, or [.., D/2] nibble-packed int8; k_scale / v_scale (and k_zp / v_zp) fp16
+    [num_pages,Hkv,page_size,G] (None for fp16 pages); token s of row b is row s % page_size of page
+    block_table[b, s // page_size] (int32 [B,P]; entries behind a row's last token are not read); context_lens int32 [B].
+
+    With `window` only the last `window` tokens and the first `sinks` are attended.  `max_ctx` bounds every context length
+    (default P * page_size); lengths are clamped to [0, max_ctx] on the device and a row of length 0 gives zeros.  No host
+    synchronisation, capturable into a CUDA graph.  A needed table entry outside the pool raises bit 3 of
+    kvq_debug_error_flag (the row is then meaningless; nothing outside the pool is read)."""
+    return _span(q, k_pages, v_pages, k_scale, v_scale, context_lens, sm_scale, block_table=block_table, window=window,
+                 sinks=sinks, max_ctx=max_ctx, k_zp=k_zp, v_zp=v_zp, inv_tau=inv_tau, out=out)
+
+
+def decode_attn_window(q, k_cache, v_cache, k_scale, v_scale, context_lens, window: int, sinks: int = 0,
+                       sm_scale: Optional[float] = None, *, k_zp=None, v_zp=None,
+                       inv_tau: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None):
+    """Sliding-window attention of one new token per row over a contiguous cache [B,Hkv,S,.] (formats as in
+    `decode_attn_paged`): of the first context_lens[b] tokens the last `window` (the newest included) and the first `sinks`
+    are attended; the rest of the cache is not read and may hold anything.  `context_lens=None`: every row has S tokens."""
+    if window is None:
+        raise ValueError("decode_attn_window needs a window; decode_attn_int8 / _int4 / _fp16 attend the whole cache")
+    return _span(q, k_cache, v_cache, k_scale, v_scale, context_lens, sm_scale, window=window, sinks=sinks, k_zp=k_zp,
+                 v_zp=v_zp, inv_tau=inv_tau, out=out)
+
+
+def decode_attn_weights(q, k_cache, v_cache, k_scale, v_scale, context_lens, weights, sm_scale: Optional[float] = None, *,
+                        k_zp=None, v_zp=None, inv_tau: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None):
+    """Attention of one new token per row over a contiguous cache [B,Hkv,S,.], which also adds the attention weights to
+    `weights` (fp32 [B,Hkv,>=S], in place): weights[b,k,s] += sum over the query heads of kv head k of their softmax weight
+    of token s, s < context_lens[b].  `evict_tokens` ranks tokens by these sums.  Deterministic: no atomics."""
+    if weights is None:
+        raise ValueError("decode_attn_weights needs a weights tensor")
+    return _span(q, k_cache, v_cache, k_scale, v_scale, context_lens, sm_scale, weights=weights, k_zp=k_zp, v_zp=v_zp,
+                 inv_tau=inv_tau, out=out)
+
+
+def evict_tokens(weights, positions, lengths, seen, budget: int, buffers, *, sinks: int = 0, recent: int = 0):
+    """Shrink every (batch row, kv head) of a contiguous cache to `budget` tokens, in place; returns the new lengths
+    (int32 [B], min(lengths, budget)).
+
+    weights fp32 [B,Hkv,S] are the accumulated attention weights, positions int32 [B,Hkv,S] the position of each slot's
+    token in the sequence (-1: appended since the last eviction, i.e. seen[b] - lengths[b] + slot; fill with -1 to start),
+    lengths / seen int32 [B] the cached tokens and all tokens a row has seen, buffers the cache tensors [B,Hkv,>=S,...] to
+    move along (payloads, scales, zero-points).  Kept: the first `sinks` and the last `recent` positions, then the largest
+    weights (equal ones: lowest slot first; NaN counts as -inf).  Kept tokens in slots below the budget stay, the others
+    fill the freed slots in ascending order: the order in the cache changes, which attention over rotated keys does not
+    see.  weights and positions follow; slots budget..lengths-1 get weight 0 and position -1.  Rows that fit stay as they
+    are."""
+    return ops.evict(weights, positions, lengths, seen, budget, buffers, sinks=sinks, recent=recent)

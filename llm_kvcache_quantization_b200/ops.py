@@ -561,3 +561,305 @@ def decode_attn_static(fmt: int, q: torch.Tensor, k_payload: torch.Tensor, v_pay
         rc = _lib.load().kvq_decode_attn_static(C.byref(a), _stream_ptr(dev))
     _lib.check("kvq_decode_attn_static", rc)
     return out
+
+
+# --------------------------------------------------------------------------- bounded and paged caches
+def _scratch(nbytes: int, device) -> torch.Tensor:
+    """Scratch memory of ONE call.  From torch's allocator and not from a buffer kept per stream: a call inside a graph
+    capture gets memory of that graph's pool, so graphs captured on one stream do not share it when they are replayed
+    side by side."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def cache_format(payload: torch.Tensor, head_dim: int) -> int:
+    """Payload format by dtype and width: fp16 [.., D], int8 [.., D], or nibble-packed [.., D/2]."""
+    if payload.dtype == torch.float16:
+        if payload.shape[-1] != head_dim:
+            raise ValueError(f"Head dim mismatch: q={head_dim}, cache={payload.shape[-1]}")
+        return FMT_FP16
+    if payload.dtype != torch.int8:
+        raise ValueError(f"cache payload must be torch.float16 or torch.int8, got {payload.dtype}")
+    if payload.shape[-1] == head_dim:
+        return FMT_INT8
+    if payload.shape[-1] * 2 == head_dim:
+        return FMT_INT4
+    raise ValueError(f"Head dim mismatch: q={head_dim}, int8 payload width {payload.shape[-1]} "
+                     "(expected head_dim, or head_dim / 2 for packed INT4)")
+
+
+def _check_pool(fmt: int, head_dim: int, k, v, k_scale, v_scale, k_zp, v_zp) -> int:
+    """Shapes, types and layout of one cache (contiguous or pool); returns the group size."""
+    if k.ndim != 4 or v.ndim != 4:
+        raise ValueError(f"cache payload must be 4D, got {tuple(k.shape)} / {tuple(v.shape)}")
+    if k.shape != v.shape or k.dtype != v.dtype:
+        raise ValueError(f"k/v cache mismatch: {tuple(k.shape)} {k.dtype} vs {tuple(v.shape)} {v.dtype}")
+    for name, t in (("k", k), ("v", v)):
+        es = t.element_size()
+        if t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise ValueError(f"{name} cache inner dim must be contiguous (stride=1), got stride={t.stride(-1)}")
+        if t.data_ptr() % 16 or any(t.stride(d) * es % 16 for d in range(3) if t.shape[d] > 1):
+            raise ValueError(f"{name} cache rows must start on 16-byte boundaries, got strides {t.stride()}")
+    if fmt == FMT_FP16:
+        if any(t is not None for t in (k_scale, v_scale, k_zp, v_zp)):
+            raise ValueError("an fp16 cache has no scales and no zero-points")
+        return head_dim
+    if k_scale is None or v_scale is None:
+        raise ValueError("a quantized cache needs k_scale and v_scale")
+    if (k_zp is None) != (v_zp is None):
+        raise ValueError("k_zp and v_zp go together")
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale), ("k_zp", k_zp), ("v_zp", v_zp)):
+        if t is None:
+            continue
+        if t.dtype != torch.float16 or t.ndim != 4 or t.shape[:3] != k.shape[:3]:
+            raise ValueError(f"{name} must be fp16 with the leading shape of the cache {tuple(k.shape[:3])}, "
+                             f"got {t.dtype} {tuple(t.shape)}")
+        if t.shape[3] > 1 and t.stride(3) != 1:
+            raise ValueError(f"{name} must be contiguous in its groups")
+    groups = k_scale.shape[3]
+    if v_scale.shape[3] != groups:
+        raise ValueError(f"k_scale/v_scale num_groups mismatch: k={groups} vs v={v_scale.shape[3]}.")
+    if groups <= 0 or head_dim % groups or (head_dim // groups) % 8:
+        raise ValueError(f"head_dim {head_dim} must be a multiple of num_groups {groups} with groups of a multiple of 8 channels")
+    for z, s in ((k_zp, k_scale), (v_zp, v_scale)):
+        if z is not None and (z.shape != s.shape or z.stride() != s.stride()):
+            raise ValueError("zero-points must share the shape and strides of the scales")
+    return head_dim // groups
+
+
+def _int32(t: torch.Tensor, what: str, n: int) -> torch.Tensor:
+    if t.ndim != 1 or t.shape[0] != n:
+        raise ValueError(f"{what} must be 1D with one entry per batch row ({n}), got {tuple(t.shape)}")
+    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+
+
+def _page_table(table: torch.Tensor, batch: int, pool: torch.Tensor) -> _lib.KvqPageTable:
+    if table.dtype != torch.int32 or table.ndim != 2 or table.shape[0] != batch or table.shape[1] < 1:
+        raise ValueError(f"block_table must be int32 [B={batch}, pages >= 1], got {table.dtype} {tuple(table.shape)}")
+    if table.shape[1] > 1 and table.stride(1) != 1:
+        raise ValueError("block_table rows must be contiguous")
+    if pool.shape[0] < 1 or pool.shape[2] < 1:
+        raise ValueError(f"the page pool {tuple(pool.shape)} holds no token")
+    return _lib.KvqPageTable(table.data_ptr(), table.stride(0), table.shape[1], pool.shape[2], pool.shape[0])
+
+
+def span_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor],
+              v_scale: Optional[torch.Tensor], context_lens: Optional[torch.Tensor], sm_scale: Optional[float] = None, *,
+              k_zp=None, v_zp=None, block_table: Optional[torch.Tensor] = None, window: Optional[int] = None, sinks: int = 0,
+              weights: Optional[torch.Tensor] = None, max_ctx: Optional[int] = None,
+              inv_tau: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """q_len == 1 attention over the visible span of a contiguous cache [B, Hkv, S, .] or, with `block_table`, of page
+    pools [num_pages, Hkv, page_size, .] (`kvq_span_attn`).  No host synchronisation: lengths are clamped on the device."""
+    dev = _require_cuda(q, k, v, k_scale, v_scale, k_zp, v_zp, context_lens, block_table, weights, inv_tau, out)
+    if q.ndim != 3:
+        raise ValueError(f"q must have shape [B, Hq, D], got {tuple(q.shape)}")
+    if q.dtype != torch.float16:
+        raise ValueError("span_attn expects an fp16 query")
+    B, Hq, D = q.shape
+    if D not in (64, 128, 256):
+        raise ValueError(f"head_dim must be 64, 128 or 256, got {D}")
+    fmt = cache_format(k, D)
+    gs = _check_pool(fmt, D, k, v, k_scale, v_scale, k_zp, v_zp)
+    Hkv = k.shape[1]
+    if Hkv < 1 or Hq % Hkv != 0:
+        raise ValueError(f"GQA head mismatch: q_heads={Hq} must be a multiple of kv_heads={Hkv}")
+    if window is None:
+        if sinks:
+            raise ValueError("sinks go with a window")
+        window = 0
+    elif window < 1 or sinks < 0:
+        raise ValueError(f"window must be >= 1 and sinks >= 0, got {window}, {sinks}")
+    s = _lib.KvqSpanAttnArgs()
+    a = s.attn
+    if block_table is None:
+        if k.shape[0] != B:
+            raise ValueError(f"Batch mismatch: q={B}, k={k.shape[0]}")
+        span = k.shape[2]
+    else:
+        s.pages = _page_table(block_table, B, k)
+        span = min(block_table.shape[1] * k.shape[2], 2 ** 31 - 1)
+    if max_ctx is not None:
+        if max_ctx < 0:
+            raise ValueError(f"max_ctx must be >= 0, got {max_ctx}")
+        span = min(span, int(max_ctx))
+    if q.stride(2) != 1 or q.stride(0) % 2 or q.stride(1) % 2 or q.data_ptr() % 4:
+        q = q.clone(memory_format=torch.contiguous_format)
+    if out is None:
+        out = torch.empty((B, Hq, D), dtype=torch.float16, device=dev)
+    elif out.dtype != torch.float16 or tuple(out.shape) != (B, Hq, D) or out.stride(2) != 1:
+        raise ValueError("out must be an fp16 [B, Hq, D] tensor, contiguous in head_dim")
+    a.format, a.B, a.Hq, a.Hkv, a.D, a.group_size, a.max_ctx = fmt, B, Hq, Hkv, D, gs, span
+    a.q, a.q_stride_b, a.q_stride_h = q.data_ptr(), q.stride(0), q.stride(1)
+    a.out, a.out_stride_b, a.out_stride_h = out.data_ptr(), out.stride(0), out.stride(1)
+    a.sm_scale = 1.0 / D ** 0.5 if sm_scale is None else float(sm_scale)
+    if inv_tau is not None:
+        if inv_tau.numel() != Hq:
+            raise ValueError(f"inv_tau must have one entry per query head ({Hq}), got {tuple(inv_tau.shape)}")
+        inv_tau = inv_tau.to(torch.float32).contiguous()
+        a.inv_tau = inv_tau.data_ptr()
+    if context_lens is not None:
+        context_lens = _int32(context_lens, "context_lens", B)
+        a.context_lens = context_lens.data_ptr()
+    elif block_table is not None:
+        raise ValueError("a paged cache needs context_lens")
+    a.k = _cache_side(k, k_scale, k_zp, None)
+    a.v = _cache_side(v, v_scale, v_zp, None)
+    s.window, s.sinks = int(window), int(sinks)
+    if weights is not None:
+        if weights.dtype != torch.float32 or weights.ndim != 3 or weights.shape[:2] != (B, Hkv) or weights.shape[2] < span:
+            raise ValueError(f"weights must be fp32 [B={B}, Hkv={Hkv}, >= {span}], got {weights.dtype} {tuple(weights.shape)}")
+        if weights.shape[2] > 1 and weights.stride(2) != 1 or \
+                any(weights.shape[d] > 1 and weights.stride(d) < weights.shape[2] for d in (0, 1)):
+            raise ValueError("weights must be contiguous in its slots, with rows that do not overlap")
+        s.weights, s.w_stride_b, s.w_stride_h = weights.data_ptr(), weights.stride(0), weights.stride(1)
+    if B == 0:
+        return out
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        need = int(lib.kvq_span_attn_workspace_bytes(C.byref(s)))
+        ws = _scratch(max(need, 256), dev)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        rc = lib.kvq_span_attn(C.byref(s), _stream_ptr(dev))
+    _lib.check("kvq_span_attn", rc)
+    return out
+
+
+def paged_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                 k_scale: Optional[torch.Tensor], v_scale: Optional[torch.Tensor], block_table: torch.Tensor,
+                 start_pos: torch.Tensor, new_lens: Optional[torch.Tensor] = None, *, k_zp=None, v_zp=None,
+                 k_static=None, v_static=None, clip_percentile: float = 100.0) -> None:
+    """Quantize new tokens [B, Hkv, T, D] into pages, one launch (`kvq_paged_append`): token t of row b goes to position
+    start_pos[b] + t of the row, t < new_lens[b] (default: all).  Scales: min / max with zero-points when zero-point pools
+    are given, the static tables [Hkv, G] when those are given, else the `clip_percentile` of each group's magnitudes."""
+    dev = _require_cuda(k_new, v_new, k_pages, v_pages, k_scale, v_scale, k_zp, v_zp, block_table, start_pos, new_lens,
+                        k_static, v_static)
+    if k_new.ndim != 4 or k_new.shape != v_new.shape:
+        raise ValueError(f"k/v shape mismatch or not 4D: {tuple(k_new.shape)} vs {tuple(v_new.shape)}")
+    B, H, T, D = k_new.shape
+    fmt = cache_format(k_pages, D)
+    gs = _check_pool(fmt, D, k_pages, v_pages, k_scale, v_scale, k_zp, v_zp)
+    if k_pages.shape[1] != H:
+        raise ValueError(f"heads mismatch: new tokens {H}, pages {k_pages.shape[1]}")
+    if (k_static is None) != (v_static is None):
+        raise ValueError("k_static and v_static go together")
+    if k_static is not None and (k_zp is not None or fmt == FMT_FP16):
+        raise ValueError("static scales are for symmetric quantized pages")
+    if not 0.0 < clip_percentile <= 100.0:
+        raise ValueError(f"clip_percentile must be in (0, 100], got {clip_percentile}")
+    for name, t in (("k_static", k_static), ("v_static", v_static)):
+        if t is not None and (tuple(t.shape) != (H, D // gs) or t.dtype not in (torch.float16, torch.float32)
+                              or not t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous fp16/fp32 [Hkv={H}, G={D // gs}] tensor, got {t.dtype} {tuple(t.shape)}")
+    k_new, v_new = k_new.to(torch.float16), v_new.to(torch.float16)
+    if k_new.stride(3) != 1:
+        k_new = k_new.contiguous()
+    if v_new.stride(3) != 1:
+        v_new = v_new.contiguous()
+    p = _lib.KvqPagedAppendArgs()
+    p.pages = _page_table(block_table, B, k_pages)
+    start_pos = _int32(start_pos, "start_pos", B)
+    p.start_pos = start_pos.data_ptr()
+    if new_lens is not None:
+        new_lens = _int32(new_lens, "new_lens", B)
+        p.new_lens = new_lens.data_ptr()
+    a = p.append
+    a.format, a.B, a.Hkv, a.T, a.D, a.group_size = fmt, B, H, T, D, gs
+    a.adaptive_margin = 1.0
+    a.quantile = clip_percentile / 100.0 if clip_percentile < 100.0 else 1.0
+    a.policy = SCALE_STATIC if fmt == FMT_FP16 or k_static is not None else \
+        SCALE_ASYM_MINMAX if k_zp is not None else SCALE_DYNAMIC_PCT
+    a.k = _append_side(k_new, k_pages, k_scale, k_zp, None, None, k_static, None)
+    a.v = _append_side(v_new, v_pages, v_scale, v_zp, None, None, v_static, None)
+    with torch.cuda.device(dev):
+        rc = _lib.load().kvq_paged_append(C.byref(p), _stream_ptr(dev))
+    _lib.check("kvq_paged_append", rc)
+
+
+def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: Optional[torch.Tensor],
+               v_scale: Optional[torch.Tensor], block_table: torch.Tensor, start_pos: Optional[torch.Tensor], tokens: int,
+               lens: Optional[torch.Tensor] = None, *, head_dim: int, k_zp=None, v_zp=None
+               ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Tokens start_pos[b] + t (default start 0), t < lens[b] (default `tokens`), of every row as fp16 (k, v)
+    [B, Hkv, tokens, head_dim]; zeros behind lens[b] (`kvq_paged_read`).  Values are code * scale (+ zero-point), rounded
+    once.  `head_dim` tells nibble-packed pages (width head_dim / 2) from INT8 ones."""
+    dev = _require_cuda(k_pages, v_pages, k_scale, v_scale, k_zp, v_zp, block_table, start_pos, lens)
+    D, T = int(head_dim), int(tokens)
+    if D not in (64, 128, 256):
+        raise ValueError(f"head_dim must be 64, 128 or 256, got {D}")
+    if T < 0:
+        raise ValueError(f"tokens must be >= 0, got {T}")
+    fmt = cache_format(k_pages, D)
+    gs = _check_pool(fmt, D, k_pages, v_pages, k_scale, v_scale, k_zp, v_zp)
+    B, H = block_table.shape[0], k_pages.shape[1]
+    p = _lib.KvqPagedReadArgs()
+    p.pages = _page_table(block_table, B, k_pages)
+    p.format, p.B, p.Hkv, p.T, p.D, p.group_size = fmt, B, H, T, D, gs
+    if start_pos is not None:
+        start_pos = _int32(start_pos, "start_pos", B)
+        p.start_pos = start_pos.data_ptr()
+    if lens is not None:
+        lens = _int32(lens, "lens", B)
+        p.lens = lens.data_ptr()
+    p.k = _cache_side(k_pages, k_scale, k_zp, None)
+    p.v = _cache_side(v_pages, v_scale, v_zp, None)
+    k = torch.empty((B, H, T, D), dtype=torch.float16, device=dev)
+    v = torch.empty_like(k)
+    if k.numel() == 0:
+        return k, v
+    p.k_out, p.v_out = k.data_ptr(), v.data_ptr()
+    p.out_stride_b, p.out_stride_h, p.out_stride_t = k.stride(0), k.stride(1), k.stride(2)
+    with torch.cuda.device(dev):
+        rc = _lib.load().kvq_paged_read(C.byref(p), _stream_ptr(dev))
+    _lib.check("kvq_paged_read", rc)
+    return k, v
+
+
+def evict(weights: torch.Tensor, positions: torch.Tensor, lengths: torch.Tensor, seen: torch.Tensor, budget: int, buffers,
+          *, sinks: int = 0, recent: int = 0) -> torch.Tensor:
+    """Shrink every (batch row, kv head) of a contiguous cache to `budget` tokens, in place (`kvq_evict`); returns the new
+    lengths, int32 [B]."""
+    buffers = tuple(buffers)
+    dev = _require_cuda(weights, positions, lengths, seen, *buffers)
+    if weights.dtype != torch.float32 or weights.ndim != 3:
+        raise ValueError(f"weights must be fp32 [B, Hkv, slots], got {weights.dtype} {tuple(weights.shape)}")
+    if positions.dtype != torch.int32 or positions.shape != weights.shape:
+        raise ValueError(f"positions must be int32 {tuple(weights.shape)}, got {positions.dtype} {tuple(positions.shape)}")
+    B, H, cap = weights.shape
+    for name, t in (("weights", weights), ("positions", positions)):
+        if (cap > 1 and t.stride(2) != 1) or any(t.shape[d] > 1 and t.stride(d) < cap for d in (0, 1)):
+            raise ValueError(f"{name} must be contiguous in its slots, with rows that do not overlap")
+    budget, sinks, recent = int(budget), int(sinks), int(recent)
+    if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
+        raise ValueError(f"need budget >= 1 and 0 <= sinks + recent <= budget, got {budget}, {sinks}, {recent}")
+    if len(buffers) > _lib.EVICT_MAX_BUFS:
+        raise ValueError(f"at most {_lib.EVICT_MAX_BUFS} buffers, got {len(buffers)}")
+    e = _lib.KvqEvictArgs()
+    e.B, e.Hkv, e.cap, e.budget, e.sinks, e.recent = B, H, cap, budget, sinks, recent
+    for i, t in enumerate(buffers):
+        if t.ndim < 3 or t.shape[:2] != (B, H) or t.shape[2] < cap:
+            raise ValueError(f"buffer {i} must be [B={B}, Hkv={H}, >= {cap} slots, ...], got {tuple(t.shape)}")
+        row = 1
+        for d in range(t.ndim - 1, 2, -1):
+            if t.shape[d] > 1 and t.stride(d) != row:
+                raise ValueError(f"buffer {i}: the row of a slot must be contiguous")
+            row *= t.shape[d]
+        if any(t.shape[d] > 1 and t.stride(d) < row for d in range(3)):
+            raise ValueError(f"buffer {i}: rows must not overlap, got strides {t.stride()}")
+        if row == 0:
+            raise ValueError(f"buffer {i} has empty rows: {tuple(t.shape)}")
+        es = t.element_size()
+        e.bufs[i] = _lib.KvqEvictBuf(t.data_ptr(), t.stride(0) * es, t.stride(1) * es, t.stride(2) * es, row * es)
+    e.n_bufs = len(buffers)
+    lengths, seen = _int32(lengths, "lengths", B), _int32(seen, "seen", B)
+    new = torch.empty(B, dtype=torch.int32, device=dev)
+    if B == 0 or H == 0:
+        return new
+    e.lengths, e.seen, e.new_lengths = lengths.data_ptr(), seen.data_ptr(), new.data_ptr()
+    e.weights, e.w_stride_b, e.w_stride_h = weights.data_ptr(), weights.stride(0), weights.stride(1)
+    e.positions, e.p_stride_b, e.p_stride_h = positions.data_ptr(), positions.stride(0), positions.stride(1)
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        ws = _scratch(int(lib.kvq_evict_workspace_bytes(B, H, cap, budget)), dev)
+        e.workspace, e.workspace_bytes = ws.data_ptr(), ws.numel()
+        rc = lib.kvq_evict(C.byref(e), _stream_ptr(dev))
+    _lib.check("kvq_evict", rc)
+    return new

@@ -32,6 +32,8 @@ class GraphedKVStackStep:
                  capacity: Optional[int] = None, overlap_append: Optional[bool] = None):
         if not isinstance(cache, (INT8KVCache, INT4KVCache, FP16KVCache)):
             raise TypeError("GraphedKVStackStep needs one of this package's caches")
+        if cache._window is not None or cache._evict is not None:
+            raise ValueError("GraphedKVStackStep attends the whole cache: it takes no attention window and no eviction")
         self.cache = cache
         L = cache.num_layers
         b0 = cache._bufs[0]
