@@ -7,6 +7,12 @@
 
 namespace kvq {
 
+// cuTensorMapEncodeTiled, resolved at run time (the library links against the runtime only); nullptr if there is none
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_tiled_fn();
+
 constexpr int kWaitLimit = 1 << 22;  // bounded mbarrier polling
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -102,6 +108,75 @@ __device__ __forceinline__ float fast_exp2(float x) {
 }
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
     return h2_as_u32(__floats2half2_rn(lo, hi));
+}
+
+// fp16 scales of the token pair (tok, tok+1), `NG` groups each, re-paired per group:
+// out[G] = half2(s[tok][G], s[tok+1][G]); `addr` = shared address of s[tok][0]
+template <int NG>
+__device__ __forceinline__ void load_scale_pairs(uint32_t addr, uint32_t (&out)[NG], uint32_t mask) {
+    if (NG == 1) {
+        uint32_t w;
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(addr));
+        out[0] = w & mask;
+    } else if (NG == 2) {
+        uint32_t r[2];
+        lds64(addr, r);
+        out[0] = prmt(r[0], r[1], 0x5410u) & mask;
+        out[NG - 1] = prmt(r[0], r[1], 0x7632u) & mask;
+    } else if (NG == 4) {
+        uint32_t r[4];
+        lds128(addr, r);
+        out[0] = prmt(r[0], r[2], 0x5410u) & mask; out[1 % NG] = prmt(r[0], r[2], 0x7632u) & mask;
+        out[2 % NG] = prmt(r[1], r[3], 0x5410u) & mask; out[3 % NG] = prmt(r[1], r[3], 0x7632u) & mask;
+    } else {
+        uint32_t ra[4], rb[4];
+        lds128(addr, ra);
+        lds128(addr + 16, rb);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            out[(2 * w) % NG] = prmt(ra[w], rb[w], 0x5410u) & mask;
+            out[(2 * w + 1) % NG] = prmt(ra[w], rb[w], 0x7632u) & mask;
+        }
+    }
+}
+// the NG fp16 values of one token row as floats; `addr` = shared address of s[row][0]
+template <int NG>
+__device__ __forceinline__ void load_row_floats(uint32_t addr, float (&f)[NG]) {
+    if (NG == 1) {
+        unsigned short u;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(addr));
+        f[0] = __half2float(__ushort_as_half(u));
+    } else if (NG == 2) {
+        uint32_t w;
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(addr));
+        const float2 v = __half22float2(u32_as_h2(w));
+        f[0] = v.x; f[NG - 1] = v.y;
+    } else {
+        uint32_t r[2];
+        lds64(addr, r);
+        const float2 a = __half22float2(u32_as_h2(r[0])), b = __half22float2(u32_as_h2(r[1]));
+        f[0] = a.x; f[1 % NG] = a.y; f[2 % NG] = b.x; f[3 % NG] = b.y;
+    }
+}
+
+constexpr uint32_t kMagic = 0x64006400u;     // half2(1024, 1024)
+constexpr uint32_t kH1152 = 0x64806480u;     // half2(1152, 1152)
+constexpr uint32_t kH1032 = 0x64086408u;     // half2(1032, 1032)
+constexpr uint32_t kHsixteenth = 0x2c002c00u;  // half2(1/16, 1/16)
+constexpr uint32_t kHm72 = 0xd480d480u;      // half2(-72, -72)
+
+// int8 pair -> exact fp16 pair.  `w` already has its sign bits flipped (w ^ 0x80808080), so
+// a byte b holds code + 128 and 0x6400 | b is the fp16 number 1152 + code.
+__device__ __forceinline__ uint32_t i8pair_to_h2(uint32_t w, uint32_t sel) {
+    return hsub2_u(prmt(w, 0x64646464u, sel), kH1152);
+}
+// two nibbles (bits 0-3 of each 16-bit half) -> exact fp16 (nibble - 8)
+__device__ __forceinline__ uint32_t nib_lo_to_h2(uint32_t w) {
+    return hsub2_u(lop3<0xEA>(w, 0x000F000Fu, kMagic), kH1032);            // (w & m) | magic
+}
+// two nibbles in bits 4-7 of each half: (1024 + 16 n) / 16 - 72 = n - 8, exact in one fma
+__device__ __forceinline__ uint32_t nib_hi_to_h2(uint32_t w) {
+    return hfma2_u(lop3<0xEA>(w, 0x00F000F0u, kMagic), kHsixteenth, kHm72);
 }
 
 }  // namespace kvq

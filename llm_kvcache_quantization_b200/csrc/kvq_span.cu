@@ -2,10 +2,14 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <math.h>
 #include <stdlib.h>
+
+#include <atomic>
 
 #include "kvq_internal.h"
 #include "kvq_span.cuh"
+#include "kvq_span_mma.cuh"
 
 namespace kvq {
 
@@ -36,6 +40,129 @@ static int max_visible_tiles(const SpanParams& p, int ts) {
     const long long t = (snk + ts - 1) / ts + (win + ts - 1) / ts + 1;       // a window may start inside a tile
     const long long all = (ctx + ts - 1) / ts;
     return (int)(t < all ? t : all);
+}
+
+// ---- tensor-core kernel: eligibility, launch configuration, tensor maps
+template <int FMT, bool ASYM, int GS, int D>
+struct SpanTag {};
+
+// Calls f(SpanTag<...>{}) for the instantiation of these arguments; KVQ_EUNSUPPORTED if there is none.
+template <class F>
+static int span_dispatch(const SpanParams& p, bool asym, F&& f) {
+    const int fmt = p.a.format, gs = p.a.group_size, d = p.a.D;
+#define KVQ_SPAN_CASE(FMT_, ASYM_, GS_, D_) \
+    if (fmt == FMT_ && asym == ASYM_ && gs == GS_ && d == D_) return f(SpanTag<FMT_, ASYM_, GS_, D_>{});
+#define KVQ_SPAN_GS(FMT_, ASYM_)                                                                                         \
+    KVQ_SPAN_CASE(FMT_, ASYM_, 32, 128) KVQ_SPAN_CASE(FMT_, ASYM_, 64, 128) KVQ_SPAN_CASE(FMT_, ASYM_, 128, 128)         \
+    KVQ_SPAN_CASE(FMT_, ASYM_, 32, 64) KVQ_SPAN_CASE(FMT_, ASYM_, 64, 64)
+    KVQ_SPAN_CASE(KVQ_FMT_FP16, false, 128, 128)
+    KVQ_SPAN_CASE(KVQ_FMT_FP16, false, 64, 64)
+    KVQ_SPAN_GS(KVQ_FMT_INT8, false)
+    KVQ_SPAN_GS(KVQ_FMT_INT8, true)
+    KVQ_SPAN_GS(KVQ_FMT_INT4, false)
+    KVQ_SPAN_GS(KVQ_FMT_INT4, true)
+#undef KVQ_SPAN_GS
+#undef KVQ_SPAN_CASE
+    return KVQ_EUNSUPPORTED;
+}
+
+static int span_stages() {
+    static const int v = [] {
+        const char* e = getenv("KVQ_SPAN_STAGES");
+        const int n = e ? atoi(e) : 2;
+        return n >= 2 && n <= kSpanMaxStages ? n : 2;
+    }();
+    return v;
+}
+
+template <int FMT, bool ASYM, int GS, int D>
+static int span_ctas_per_sm(SpanTag<FMT, ASYM, GS, D>, int& out) {
+    // once per device: the shared-memory limit is an attribute of the function on that device
+    static std::atomic<int> cached[64];
+    int dev = 0;
+    int rc = check_cuda(cudaGetDevice(&dev));
+    if (rc) return rc;
+    if (dev < 0 || dev >= 64) return KVQ_EUNSUPPORTED;
+    int n = cached[dev].load(std::memory_order_relaxed);
+    if (n == 0) {
+        const size_t smem = SpanShape<FMT, ASYM, GS, D>::smem(span_stages());
+        rc = check_cuda(cudaFuncSetAttribute(span_mma_kernel<FMT, ASYM, GS, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        if (rc) return rc;
+        rc = check_cuda(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, span_mma_kernel<FMT, ASYM, GS, D>, kSpanWarps * 32, smem));
+        if (rc) return rc;
+        if (n < 1) n = 1;
+        cached[dev].store(n, std::memory_order_relaxed);
+    }
+    out = n;
+    return KVQ_OK;
+}
+
+// Payload as (row bytes in 128-byte rows of `tpr` tokens, token rows, kv heads, batch rows or pages); box = 128 bytes x
+// box_rows.  Rows at or beyond the extent are zero-filled by the copy engine.
+static int span_map(CUtensorMap* map, const KvqCacheSide& sd, const KvqAttnArgs& a, const KvqPageTable& pg, int rb, int tpr, int box_rows) {
+    EncodeTiledFn enc = encode_tiled_fn();
+    if (!enc) return KVQ_EUNSUPPORTED;
+    const int tokens = pg.table ? pg.page_size : a.max_ctx, major = pg.table ? pg.num_pages : a.B;
+    const cuuint64_t rs = (cuuint64_t)tpr * sd.pay_stride_s;
+    cuuint64_t dims[4] = {(cuuint64_t)(rb < 128 ? 128 : rb), (cuuint64_t)(tokens / tpr), (cuuint64_t)a.Hkv, (cuuint64_t)major};
+    // a dimension of extent 1 never advances: any legal stride
+    cuuint64_t strides[3] = {rs, a.Hkv > 1 ? (cuuint64_t)sd.pay_stride_h : rs, major > 1 ? (cuuint64_t)sd.pay_stride_b : rs};
+    cuuint32_t box[4] = {128, (cuuint32_t)box_rows, 1, 1};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(sd.payload), dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? KVQ_OK : KVQ_EUNSUPPORTED;
+}
+
+// Tokens of one payload copy, 0 if the kernel cannot take the layout.  A copy must not cross a page, and must be at least
+// 1024 bytes (the period of the swizzle).
+template <int FMT, bool ASYM, int GS, int D>
+static int span_box(SpanTag<FMT, ASYM, GS, D>, const SpanParams& p) {
+    using S = SpanShape<FMT, ASYM, GS, D>;
+    int box = S::TS;
+    if (p.pg.table)
+        while (box >= 16 && p.pg.page_size % box) box /= 2;
+    return box >= 16 && box * (S::RB < 128 ? S::RB : 128) >= 1024 ? box : 0;
+}
+
+template <int FMT, bool ASYM, int GS, int D>
+static int span_tile(SpanTag<FMT, ASYM, GS, D>) { return SpanShape<FMT, ASYM, GS, D>::TS; }
+
+static bool span_mma_side(const KvqCacheSide& s, const SpanParams& p, int rb, int tpr, int ng) {
+    const KvqAttnArgs& a = p.a;
+    const int major = p.pg.table ? p.pg.num_pages : a.B;
+    if (s.pay_stride_s < rb || (tpr > 1 && s.pay_stride_s != rb)) return false;
+    if ((a.Hkv > 1 && s.pay_stride_h <= 0) || (major > 1 && s.pay_stride_b <= 0)) return false;
+    if (s.pay_stride_s >= (1LL << 36) || s.pay_stride_h >= (1LL << 40) || s.pay_stride_b >= (1LL << 40)) return false;
+    if (ng == 0) return true;
+    if (s.sc_stride_s != ng || (a.Hkv > 1 && (s.sc_stride_h & 7)) || (major > 1 && (s.sc_stride_b & 7))) return false;
+    return !(((uintptr_t)s.scale | (uintptr_t)s.zp) & 15);
+}
+
+template <int FMT, bool ASYM, int GS, int D>
+static bool span_mma_ok(SpanTag<FMT, ASYM, GS, D> tag, const SpanParams& p) {
+    using S = SpanShape<FMT, ASYM, GS, D>;
+    const KvqAttnArgs& a = p.a;
+    if (getenv("KVQ_FORCE_GENERIC") || a.max_ctx < S::TPR) return false;
+    if (!(fabsf(a.sm_scale) > 0.f && fabsf(a.sm_scale) <= 1e30f)) return false;      // masked logits are -inf before the scale
+    const int ng = S::F16 ? 0 : S::NG;
+    return span_box(tag, p) && span_mma_side(a.k, p, S::RB, S::TPR, ng) && span_mma_side(a.v, p, S::RB, S::TPR, ng);
+}
+
+template <int FMT, bool ASYM, int GS, int D>
+static int launch_span_mma(SpanTag<FMT, ASYM, GS, D> tag, const SpanParams& p, cudaStream_t st) {
+    using S = SpanShape<FMT, ASYM, GS, D>;
+    SpanMmaParams mp;
+    mp.p = p;
+    mp.nstage = span_stages();
+    mp.box_tokens = span_box(tag, p);
+    CUtensorMap kmap, vmap;
+    int rc, n;
+    if ((rc = span_ctas_per_sm(tag, n))) return rc;
+    if ((rc = span_map(&kmap, p.a.k, p.a, p.pg, S::RB, S::TPR, mp.box_tokens / S::TPR))) return rc;
+    if ((rc = span_map(&vmap, p.a.v, p.a, p.pg, S::RB, S::TPR, mp.box_tokens / S::TPR))) return rc;
+    return launch_pdl(span_mma_kernel<FMT, ASYM, GS, D>, dim3(p.ctas), dim3(kSpanWarps * 32), S::smem(mp.nstage), st, mp, kmap, vmap);
 }
 
 static int span_plan(const KvqSpanAttnArgs& s, SpanPlan& pl) {
@@ -71,10 +198,19 @@ static int span_plan(const KvqSpanAttnArgs& s, SpanPlan& pl) {
     p.w_stride_h = s.w_stride_h;
     pl.kind = 0;
     pl.ts = kSpanGenericTS;
+    int slots = device_sm_count() * 4;
+    span_dispatch(p, pl.asym, [&](auto tag) {
+        if (!span_mma_ok(tag, p)) return KVQ_OK;
+        int n = 1;
+        if (span_ctas_per_sm(tag, n)) n = 1;               // no device: the launch will say so
+        pl.kind = 1;
+        pl.ts = span_tile(tag);
+        slots = device_sm_count() * n;
+        return KVQ_OK;
+    });
     pl.rows = (long long)a.B * p.hr;
     const long long per_row = max_visible_tiles(p, pl.ts);
     if (pl.rows * per_row >= (1LL << 31) || pl.rows >= (1LL << 30) || a.B > 65535) return KVQ_ELIMIT;
-    int slots = device_sm_count() * 4;
     // A run of fewer than 4 tiles leaves warps of the CTA without work; a row of at most 8 tiles (two per warp) is
     // not worth cutting: it takes one CTA, and the join is saved.
     p.min_tiles = 4;
@@ -163,8 +299,9 @@ extern "C" int kvq_span_attn(const KvqSpanAttnArgs* args, kvq_stream_t stream) {
     p.fin = p.weights ? (float*)(ws + pl.o_bytes + pl.ml_bytes) : nullptr;
     p.logits = p.weights ? (float*)(ws + pl.o_bytes + pl.ml_bytes + pl.fin_bytes) : nullptr;
     cudaStream_t st = (cudaStream_t)stream;
-    if ((rc = span_generic(pl, st))) return rc;
-    if (!p.row_mode && (rc = span_join<kSpanGenericTS>(p, st))) return rc;
+    rc = pl.kind ? span_dispatch(p, pl.asym, [&](auto tag) { return launch_span_mma(tag, p, st); }) : span_generic(pl, st);
+    if (rc) return rc;
+    if (!p.row_mode && (rc = pl.ts == 64 ? span_join<64>(p, st) : span_join<32>(p, st))) return rc;
     if (p.weights && a.max_ctx > 0)
         rc = launch_pdl(span_weights_kernel, dim3((a.max_ctx + 255) / 256, a.Hkv, a.B), dim3(256), 0, st, p);
     return rc;

@@ -7,7 +7,7 @@ import torch
 
 import llm_kvcache_quantization_b200 as kvq
 from llm_kvcache_quantization_b200 import _lib, ops
-from span_reference import attention, check, evict, make_cache, make_table, paginate, values
+from span_reference import attention, check, evict, make_cache, make_table, paginate, values, visible
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -32,7 +32,6 @@ def _case(B, Hq, Hkv, D, S, fmt, gs, seed):
 
 def _poison(t, lens, window=0, sinks=0):
     """NaN / extreme codes in every slot outside the visible span."""
-    from span_reference import visible
     if t is None:
         return None
     t = t.clone()
@@ -68,6 +67,10 @@ def test_paged_attention(case, fmt):
     out, tol, _, _ = attention(q, k, v, ks, vs, kz, vz, lens, window, sinks)
     pool, table = make_table(lens, page, gen)
     pages = [paginate(_poison(t, lens, window, sinks), lens, page, pool, table) for t in (k, v, ks, vs, kz, vz)]
+    for b, n in enumerate(lens):                            # pages that the window has left may be gone
+        for j in range(-(-n // page)):
+            if not visible(n, table.shape[1] * page, window, sinks)[j * page:(j + 1) * page].any():
+                table[b, j] = -1
     qd, kd, vd, ksd, vsd, kzd, vzd, td = _d(q, *pages, table)
     lend = torch.tensor(lens, dtype=torch.int32, device=DEV)
     got = kvq.decode_attn_paged(qd, kd, vd, ksd, vsd, td, lend, window=window or None, sinks=sinks, k_zp=kzd, v_zp=vzd)
@@ -128,6 +131,29 @@ def test_zero_rows_zero_context_and_empty_batch():
     empty = torch.zeros(2, 2, 0, 128, dtype=torch.float16, device=DEV)
     assert (kvq.decode_attn_window(q, empty, empty, None, None, None, 8) == 0).all()
     assert _flag() == 0
+
+
+def test_which_kernel_serves_which_layout():
+    def kind(fmt, D, gs, page, zp=False):
+        gen = torch.Generator().manual_seed(0)
+        k, ks, kz = _d(*make_cache((4, 2, page or 96), D, fmt, gs, gen))
+        s = _lib.KvqSpanAttnArgs()
+        a = s.attn
+        a.format, a.B, a.Hq, a.Hkv, a.D, a.group_size = ops.cache_format(k, D), 4, 8, 2, D, gs
+        a.sm_scale, a.max_ctx = 0.1, k.shape[2]
+        a.k = a.v = ops._cache_side(k, ks, kz, None)
+        if page:
+            s.pages = _lib.KvqPageTable(k.data_ptr(), 1, 1, page, 4)
+        return _lib.load().kvq_span_attn_kernel_kind(C.byref(s))
+    for fmt in FORMATS:
+        for D in (64, 128):
+            for gs in ((D,) if fmt == "fp16" else (32, D)):
+                for page in (0, 32, 64, 128):
+                    assert kind(fmt, D, gs, page) == 1, (fmt, D, gs, page)
+                assert kind(fmt, D, gs, 16) == (0 if fmt.startswith("int4") and D == 64 else 1)
+                assert kind(fmt, D, gs, 8) == 0
+        assert kind(fmt, 256, 128, 32) == 0
+    assert kind("int8", 128, 16, 32) == 0
 
 
 # ------------------------------------------------------------------------------------------------ window
@@ -588,7 +614,8 @@ def test_contiguous_cache_with_eviction(kind):
         c.append(0, *(torch.randn(B, H, new, D, generator=gen).half().to(DEV) for _ in range(2)))
         seen += new
         n = c.get_seq_len()
-        bufs = {m: t[:, :, :n].cpu() for m, t in c._bufs[0].items()}
+        snap = {m: t.clone()[:, :, :n] for m, t in c._bufs[0].items()}         # same strides: the same kernel serves them
+        bufs = {m: t.cpu() for m, t in snap.items()}
         q = torch.randn(B, Hq, D, generator=gen).half()
         before = torch.zeros(B, H, n, dtype=torch.float64)
         before[:, :, :w.shape[2]] = w.double()
@@ -599,10 +626,8 @@ def test_contiguous_cache_with_eviction(kind):
         check(got, out, tol, f"step {step}")
         # the sums that the eviction saw differ from the 64-bit ones by rounding: rank by a second, identical pass
         again = before.float().to(DEV)
-        ops.span_attn(q.to(DEV), *(None if t is None else t.to(DEV) for t in
-                                   (bufs["k"], bufs["v"], bufs.get("ks"), bufs.get("vs"))), None, 1 / math.sqrt(D),
-                      weights=again, k_zp=None if kind != "int4z" else bufs["kz"].to(DEV),
-                      v_zp=None if kind != "int4z" else bufs["vz"].to(DEV))
+        ops.span_attn(q.to(DEV), snap["k"], snap["v"], snap.get("ks"), snap.get("vs"), None, 1 / math.sqrt(D),
+                      weights=again, k_zp=snap.get("kz"), v_zp=snap.get("vz"))
         check(again, before + dw, dwtol + (before + dw) * 2.0 ** -23)
         i32 = torch.full((B,), n, dtype=torch.int32)
         w, pos, lens, moves = evict(again.cpu(), pos, i32, torch.full((B,), seen, dtype=torch.int32), budget, sinks, recent)
