@@ -66,15 +66,6 @@ static int span_dispatch(const SpanParams& p, bool asym, F&& f) {
     return KVQ_EUNSUPPORTED;
 }
 
-static int span_stages() {
-    static const int v = [] {
-        const char* e = getenv("KVQ_SPAN_STAGES");
-        const int n = e ? atoi(e) : 2;
-        return n >= 2 && n <= kSpanMaxStages ? n : 2;
-    }();
-    return v;
-}
-
 template <int FMT, bool ASYM, int GS, int D>
 static int span_ctas_per_sm(SpanTag<FMT, ASYM, GS, D>, int& out) {
     // once per device: the shared-memory limit is an attribute of the function on that device
@@ -85,7 +76,7 @@ static int span_ctas_per_sm(SpanTag<FMT, ASYM, GS, D>, int& out) {
     if (dev < 0 || dev >= 64) return KVQ_EUNSUPPORTED;
     int n = cached[dev].load(std::memory_order_relaxed);
     if (n == 0) {
-        const size_t smem = SpanShape<FMT, ASYM, GS, D>::smem(span_stages());
+        const size_t smem = SpanShape<FMT, ASYM, GS, D>::smem();
         rc = check_cuda(cudaFuncSetAttribute(span_mma_kernel<FMT, ASYM, GS, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         if (rc) return rc;
         rc = check_cuda(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, span_mma_kernel<FMT, ASYM, GS, D>, kSpanWarps * 32, smem));
@@ -120,7 +111,7 @@ static int span_map(CUtensorMap* map, const KvqCacheSide& sd, const KvqAttnArgs&
 template <int FMT, bool ASYM, int GS, int D>
 static int span_box(SpanTag<FMT, ASYM, GS, D>, const SpanParams& p) {
     using S = SpanShape<FMT, ASYM, GS, D>;
-    int box = S::TS;
+    int box = S::TSW;
     if (p.pg.table)
         while (box >= 16 && p.pg.page_size % box) box /= 2;
     return box >= 16 && box * (S::RB < 128 ? S::RB : 128) >= 1024 ? box : 0;
@@ -155,14 +146,13 @@ static int launch_span_mma(SpanTag<FMT, ASYM, GS, D> tag, const SpanParams& p, c
     using S = SpanShape<FMT, ASYM, GS, D>;
     SpanMmaParams mp;
     mp.p = p;
-    mp.nstage = span_stages();
     mp.box_tokens = span_box(tag, p);
     CUtensorMap kmap, vmap;
     int rc, n;
     if ((rc = span_ctas_per_sm(tag, n))) return rc;
     if ((rc = span_map(&kmap, p.a.k, p.a, p.pg, S::RB, S::TPR, mp.box_tokens / S::TPR))) return rc;
     if ((rc = span_map(&vmap, p.a.v, p.a, p.pg, S::RB, S::TPR, mp.box_tokens / S::TPR))) return rc;
-    return launch_pdl(span_mma_kernel<FMT, ASYM, GS, D>, dim3(p.ctas), dim3(kSpanWarps * 32), S::smem(mp.nstage), st, mp, kmap, vmap);
+    return launch_pdl(span_mma_kernel<FMT, ASYM, GS, D>, dim3(p.ctas), dim3(kSpanWarps * 32), S::smem(), st, mp, kmap, vmap);
 }
 
 static int span_plan(const KvqSpanAttnArgs& s, SpanPlan& pl) {
@@ -211,10 +201,10 @@ static int span_plan(const KvqSpanAttnArgs& s, SpanPlan& pl) {
     pl.rows = (long long)a.B * p.hr;
     const long long per_row = max_visible_tiles(p, pl.ts);
     if (pl.rows * per_row >= (1LL << 31) || pl.rows >= (1LL << 30) || a.B > 65535) return KVQ_ELIMIT;
-    // A run of fewer than 4 tiles leaves warps of the CTA without work; a row of at most 8 tiles (two per warp) is
-    // not worth cutting: it takes one CTA, and the join is saved.
-    p.min_tiles = 4;
-    p.row_mode = per_row <= 8;
+    // A warp of the generic kernel takes a whole tile, so a run has at least 4; the tensor-core kernel's tiles are the CTA's.
+    // A row of at most 256 tokens is not worth cutting: it takes one CTA, and the join is saved.
+    p.min_tiles = pl.kind ? 1 : 4;
+    p.row_mode = per_row * pl.ts <= 256;
     long long ctas = (pl.rows * per_row + p.min_tiles - 1) / p.min_tiles;
     p.ctas = p.row_mode ? (int)pl.rows : (int)(ctas < slots ? ctas : slots);
     const size_t parts = p.row_mode ? 0 : (size_t)p.ctas + pl.rows;
@@ -301,7 +291,15 @@ extern "C" int kvq_span_attn(const KvqSpanAttnArgs* args, kvq_stream_t stream) {
     cudaStream_t st = (cudaStream_t)stream;
     rc = pl.kind ? span_dispatch(p, pl.asym, [&](auto tag) { return launch_span_mma(tag, p, st); }) : span_generic(pl, st);
     if (rc) return rc;
-    if (!p.row_mode && (rc = pl.ts == 64 ? span_join<64>(p, st) : span_join<32>(p, st))) return rc;
+    if (!p.row_mode) {
+        switch (pl.ts) {
+            case 32: rc = span_join<32>(p, st); break;
+            case 64: rc = span_join<64>(p, st); break;
+            case 128: rc = span_join<128>(p, st); break;
+            default: rc = span_join<256>(p, st); break;
+        }
+        if (rc) return rc;
+    }
     if (p.weights && a.max_ctx > 0)
         rc = launch_pdl(span_weights_kernel, dim3((a.max_ctx + 255) / 256, a.Hkv, a.B), dim3(256), 0, st, p);
     return rc;

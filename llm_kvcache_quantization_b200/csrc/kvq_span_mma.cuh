@@ -8,18 +8,20 @@
 //         from -offset sum_group q (the C operand of the group's first mma) and are multiplied by the token's fp32 scale
 //         afterwards.  Codes, q and products are exact; the offset costs one more bit of the fp32 sums.
 //         Zero-points add z_group sum_group q.
-//   P.V   channels on M, heads on N, tokens on K.  V codes become exact signed fp16 (a sum over 10^5 tokens would feel an
-//         offset), the V scale goes into P: for one group per token in fp32 before P is rounded to fp16 (one rounding,
-//         2^-11 of p), for several groups as a product of fp16 pairs per group (a second rounding).  V zero-points are one
-//         more mma, with the groups on M.
+//   P.V   channels on M, heads on N, tokens on K.  The V scale goes into P: for one group per token in fp32 before P is
+//         rounded to fp16 (one rounding, 2^-11 of p), for several groups as a product of fp16 pairs per group (a second
+//         rounding).  V codes enter with their offset as well; offset x sum P scale_v (one mma with a matrix of ones) is
+//         taken out after every tile, so that a sum over 10^5 tokens does not carry it along.  V zero-points are one more
+//         mma, with the groups on M.
 // Both roundings of P are relative as long as P scale_v stays in fp16's normal range, whatever the scales: probabilities are
-// kept relative to r = max logit - e, with e such that 2^e scale_v <= 2^14 (2^e <= 2^15) for the largest scale met so far.  r
-// only grows, so it takes the place of the running maximum in the online softmax and costs nothing per element.
-//
-// Copies.  Each of the 4 warps owns a ring of tiles and walks every fourth tile of the CTA's run: payload by
-// cp.async.bulk.tensor (128-byte rows, 128-byte swizzle; rows shorter than that hold 2 or 4 tokens, longer ones are fetched
-// as 2 halves), one copy per page piece of 16 / 32 / TS tokens, scales by 16-byte cp.async, all on the slot's mbarrier.  No
-// producer warp and no CTA barrier inside a row.  Waits are bounded; an expired one raises bit 0 of the error flag.
+// 2^(x - r) with r = (a maximum of the logits x so far) - e, where e keeps 2^(e+3) scale_v <= 2^15 for the largest scale met
+// so far, and r moves only when a logit exceeds it by e + 3: no maximum over the warp in most tiles.
+// Copies.  A CTA walks tiles of 4 x TSW tokens, TSW per warp, so that the K or the V part of a tile is 16 KB; the parts
+// take turns in a ring of 3 slots (4 CTAs of 4 warps fit an SM).  One warp fetches a part for all: payload by
+// cp.async.bulk.tensor (128-byte rows, 128-byte swizzle; rows shorter than that hold 2 or 4 tokens, longer ones come as 2
+// halves), one copy per page piece or warp share that has a visible token, scales by 16-byte cp.async, all on the slot's
+// mbarrier.  The warp that finishes a slot last refills it, so there is no producer warp and no barrier inside a row.  Waits
+// are bounded; an expired one raises bit 0 of the error flag.
 #pragma once
 
 #include "kvq_ptx.cuh"
@@ -28,20 +30,21 @@
 namespace kvq {
 
 constexpr int kSpanWarps = 4;
-constexpr int kSpanMaxStages = 4;
+constexpr int kSpanSlots = 3;
 
 template <int FMT, bool ASYM, int GS, int D>
 struct SpanShape {
     static constexpr bool F16 = FMT == KVQ_FMT_FP16;
     static constexpr int RB = F16 ? 2 * D : FMT == KVQ_FMT_INT8 ? D : D / 2;   // payload bytes of a token
     static constexpr int TPR = RB < 128 ? 128 / RB : 1;                        // tokens per 128-byte row
-    static constexpr int TS = RB < 128 ? 64 : 32;                              // tokens per tile
+    static constexpr int TSW = RB >= 256 ? 16 : RB == 128 ? 32 : 64;           // tokens of a warp
+    static constexpr int TS = kSpanWarps * TSW;                                // tokens of a tile
     static constexpr int NG = F16 ? 1 : D / GS;
-    static constexpr int TILE = TS * RB;                                       // bytes of K (or V) of a tile
-    static constexpr int SCB = F16 ? 0 : TS * NG * 2;                          // bytes of one scale tile
-    static constexpr int SCT = (ASYM ? 4 : 2) * SCB;
-    static constexpr size_t smem(int nstage) {
-        const size_t ring = (size_t)kSpanWarps * nstage * (2 * TILE + SCT);
+    static constexpr int TILE = TS * RB;                                       // bytes of K (or V) of a tile: a ring slot
+    static constexpr int SCB = F16 ? 0 : TS * NG * 2;                          // bytes of one scale table of a tile
+    static constexpr int SCT = (ASYM ? 2 : 1) * SCB;
+    static constexpr size_t smem() {
+        const size_t ring = (size_t)kSpanSlots * (TILE + SCT);
         const size_t red = (size_t)kSpanWarps * kHeadsPerCta * (D + 8) * 4;
         return (ring > red ? ring : red) + 1024;
     }
@@ -49,18 +52,9 @@ struct SpanShape {
 
 struct SpanMmaParams {
     SpanParams p;
-    int nstage;
-    int box_tokens;          // tokens of one payload copy: divides TS and the page
+    int box_tokens;          // tokens of one payload copy: divides TSW and the page
 };
 
-// shared-memory offset of 16-byte chunk c of token r inside a payload tile
-template <int RB, int TS>
-__device__ __forceinline__ uint32_t span_off(int r, int c) {
-    if (RB >= 128) return (uint32_t)((c >> 3) * (TS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-    constexpr int TPR = RB < 128 ? 128 / RB : 1;
-    const int row = r / TPR, cc = (r % TPR) * (RB / 16) + c;
-    return (uint32_t)(row * 128 + ((cc ^ (row & 7)) << 4));
-}
 __device__ __forceinline__ void sts128(uint32_t addr, uint4 v) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -83,128 +77,178 @@ __device__ __forceinline__ void mma16816_from(float (&c)[4], uint32_t a0, uint32
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
 }
 
+__device__ __forceinline__ uint32_t span_atom_add(uint32_t addr) {
+    uint32_t old;
+    asm volatile("atom.acq_rel.cta.shared.add.u32 %0, [%1], 1;" : "=r"(old) : "r"(addr) : "memory");
+    return old;
+}
+
 template <int FMT, bool ASYM, int GS, int D>
 __global__ void __launch_bounds__(kSpanWarps * 32, 4)
 span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     using S = SpanShape<FMT, ASYM, GS, D>;
     constexpr bool F16 = S::F16, I8 = FMT == KVQ_FMT_INT8;
-    constexpr int RB = S::RB, TPR = S::TPR, TS = S::TS, NG = S::NG, TILE = S::TILE, SCB = S::SCB, SCT = S::SCT;
-    constexpr int SUB = TS / 16, H = kHeadsPerCta;
+    constexpr int RB = S::RB, TPR = S::TPR, TS = S::TS, TSW = S::TSW, NG = S::NG, TILE = S::TILE, SCB = S::SCB, SCT = S::SCT;
+    constexpr int SUB = TSW / 16, H = kHeadsPerCta;
     constexpr int NQ = D / 8;                                  // fragment registers of q
+    constexpr int SUBSTEP = 16 * (RB < 128 ? RB : 128);        // bytes between 16-token pieces of a tile
     constexpr float OFFSET = I8 ? 128.f : 8.f;
+    constexpr float U24 = 1.f / 16777216.f;
     const SpanParams& p = mp.p;
     const KvqAttnArgs& a = p.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, t = lane & 3;
-    const int nstage = mp.nstage;
 
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* smem = smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u);
-    const uint32_t pay_u = smem_u32(smem) + (uint32_t)(warp * nstage * 2 * TILE);
-    const uint32_t sc_u = smem_u32(smem) + (uint32_t)(kSpanWarps * nstage * 2 * TILE + warp * nstage * SCT);
-    __shared__ __align__(8) unsigned long long bars[kSpanWarps][kSpanMaxStages];
+    const uint32_t ring_u = smem_u32(smem), scale_u = ring_u + kSpanSlots * TILE;
+    __shared__ __align__(8) unsigned long long bars[kSpanSlots];
+    __shared__ uint32_t done[kSpanSlots];                      // warps that have finished with a slot
     __shared__ float red_ml[kSpanWarps][H][2];
     __shared__ float red_w[kSpanWarps][H];
     __shared__ float red_tot[H][2];
     __shared__ int sh[kSpanWarps + 4];
 
-    const uint32_t bar0 = smem_u32(&bars[warp][0]);
-    if (lane == 0) {
-        for (int s = 0; s < nstage; ++s) mbar_init(bar0 + 8 * s, F16 ? 1 : 33);      // expect_tx (+ 32 cp.async arrivals)
+    const uint32_t bar0 = smem_u32(&bars[0]), done0 = smem_u32(&done[0]);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kSpanSlots; ++s) {
+            mbar_init(bar0 + 8 * s, F16 ? 1 : 33);             // expect_tx (+ 32 cp.async arrivals)
+            done[s] = 0;
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
     }
-    __syncwarp();
+    __syncthreads();
     pdl_wait();                                                // q, the cache, the lengths and the table
 
     SpanCursor cur = span_locate<TS, kSpanWarps * 32>(p, blockIdx.x, sh);
     if (cur.left == 0 && !p.row_mode) return;                  // uniform over the CTA
     RowView v = row_view<TS>(p, cur.b);
-    const float scale2 = fabsf(a.sm_scale) * kLog2e * (F16 ? 1.f : 16777216.f);      // q carries the sign; 2^24: subnormals
+    const float scale2 = fabsf(a.sm_scale) * kLog2e * (F16 ? 1.f : 1.f / U24);       // q carries the sign; subnormal codes
     const int box = mp.box_tokens, nbox = TS / box;
-    int issued = 0, taken = 0;                                 // tiles of this warp over the whole run: slot = count % nstage
-    int islot = 0, tslot = 0;
-    uint32_t tphase = 0;
+    // ldmatrix addresses of this lane inside a slot; 16-byte chunk c of token piece `sub`: (slot + base) ^ (c << 4), plus
+    // sub * SUBSTEP, plus TS * 128 for the second half of a 256-byte row
+    uint32_t lk, lv;
+    {
+        auto base = [&](int r, int hi) -> uint32_t {           // token r of the warp's share, odd chunk or not
+            if (RB >= 128) return (uint32_t)((warp * TSW + r) * 128 + ((hi ^ (r & 7)) << 4));
+            const int row = r / TPR;
+            return (uint32_t)((warp * TSW / TPR + row) * 128 + ((((r % TPR) * (RB / 16)) | hi) ^ (row & 7)) * 16);
+        };
+        lk = base(((lane >> 3) & 1) * 8 + (lane & 7), lane >> 4);
+        lv = F16 ? base((lane >> 4) * 8 + (lane & 7), (lane >> 3) & 1) : lk;
+    }
+    auto chunk_addr = [&](uint32_t lane_slot, int sub, int c) -> uint32_t {
+        uint32_t x = lane_slot ^ ((uint32_t)(c & 6) << 4);
+        if (RB == 32 && (sub & 1)) x ^= 64u;                   // four tokens a row: the swizzle's row number moves by 4
+        return x + sub * SUBSTEP + (RB > 128 ? (c >> 3) * (TS * 128) : 0);
+    };
+    int slot = 0;
+    uint32_t phase = 0;
     bool failed = false;
 
     for (;;) {
         const int b = cur.b, kvh = cur.hr / p.rep_chunks, rc = cur.hr - kvh * p.rep_chunks;
         const int h0 = kvh * p.n_rep + rc * H, nh = min(H, p.n_rep - rc * H);
         const long long row = (long long)b * p.hr + cur.hr;
-        const int i0 = cur.i + warp, i1 = min(v.tiles, cur.i + cur.left);
-        const int n_my = i0 < i1 && !failed ? (i1 - i0 + kSpanWarps - 1) / kSpanWarps : 0;
+        const int i1 = min(v.tiles, cur.i + cur.left), ntile = i1 - cur.i;
+        const int slot0 = slot;                                // slot of part 0 of this row
 
-        // ---- request tile k of this warp's list
-        auto issue = [&](int k) {
-            const int tok0 = tile_token<TS>(v, i0 + k * kSpanWarps);
-            const uint32_t pb = pay_u + islot * 2 * TILE, sb = sc_u + islot * SCT, bar = bar0 + 8 * islot;
-            if (++islot == nstage) islot = 0;
-            ++issued;
+        // ---- request part u (K of tile u / 2 for even u, V for odd u) into its slot; called by one whole warp
+        auto issue = [&](int u) {
+            const int side = u & 1, tok0 = tile_token<TS>(v, cur.i + (u >> 1));
+            const int s = (slot0 + u) % kSpanSlots;
+            const uint32_t dst = ring_u + s * TILE, sb = scale_u + s * SCT, bar = bar0 + 8 * s;
+            const KvqCacheSide& cs = side ? a.v : a.k;
             // batch row or page, and the row in it, of the piece of `box` tokens that this lane's number names
-            int page = b, prow = tok0 + lane * box;
-            if (p.pg.table) {
-                // pieces without a visible token hold nothing that is used (their pages may be gone): page 0 serves
-                const int tok = prow;
-                page = prow = 0;
-                if (lane < nbox && tok < v.n && (tok + box > v.wstart || tok < v.sinks)) {
-                    const int blk = tok / p.pg.page_size;
-                    page = __ldg(p.pg.table + b * p.pg.stride_b + blk);
-                    prow = tok - blk * p.pg.page_size;
-                    if (page < 0 || page >= p.pg.num_pages) {
-                        atomicOr(&g_span_error_flag, 2);
-                        page = 0;
-                    }
+            const int tok = tok0 + lane * box;
+            const bool vis = lane < nbox && tok < v.n && (tok + box > v.wstart || tok < v.sinks);
+            int major = b, minor = tok;
+            if (p.pg.table && vis) {
+                const int blk = tok / p.pg.page_size;
+                major = __ldg(p.pg.table + b * p.pg.stride_b + blk);
+                minor = tok - blk * p.pg.page_size;
+                if (major < 0 || major >= p.pg.num_pages) {
+                    atomicOr(&g_span_error_flag, 2);
+                    major = 0;
                 }
             }
-            if (lane == 0) mbar_expect_tx(bar, 2 * TILE);
+            const unsigned vmask = __ballot_sync(0xffffffffu, vis);
+            if (lane == 0) mbar_expect_tx(bar, __popc(vmask) * box * RB);
             __syncwarp();
-            if (lane < nbox) {
-                const uint32_t off = lane * box * (RB < 128 ? RB : 128);
-                const int y = prow / TPR;
-                tma_load_4d(pb + off, &kmap, bar, 0, y, kvh, page);
-                if (RB > 128) tma_load_4d(pb + TS * 128 + off, &kmap, bar, 128, y, kvh, page);
-                tma_load_4d(pb + TILE + off, &vmap, bar, 0, y, kvh, page);
-                if (RB > 128) tma_load_4d(pb + TILE + TS * 128 + off, &vmap, bar, 128, y, kvh, page);
+            if (vis) {
+                const CUtensorMap* map = side ? &vmap : &kmap;
+                const uint32_t d = dst + lane * box * (RB < 128 ? RB : 128);
+                tma_load_4d(d, map, bar, 0, minor / TPR, kvh, major);
+                if (RB > 128) tma_load_4d(d + TS * 128, map, bar, 128, minor / TPR, kvh, major);
             }
             if (!F16) {
-                constexpr int CH = TS * NG / 8;                // 16-byte chunks of one scale tile
+                constexpr int CH = TS * NG / 8;                // 16-byte chunks of one scale table
+                const int pieces = box * NG / 8;               // of them in a piece
 #pragma unroll
                 for (int c0 = 0; c0 < CH; c0 += 32) {
-                    const int c = c0 + lane;
-                    const int ct = c * 8 / NG;                 // first token of the chunk, relative to the tile
-                    int mj = b, mn = tok0 + ct, nbytes = 16;   // batch row or page, row, bytes inside the buffers
-                    if (p.pg.table) {
-                        const int bx = min(ct / box, nbox - 1);
-                        mj = __shfl_sync(0xffffffffu, page, bx);
-                        mn = __shfl_sync(0xffffffffu, prow, bx) + ct - bx * box;
-                    } else {
-                        nbytes = max(0, min(16, (a.max_ctx - mn) * 2 * NG));
-                        if (nbytes == 0) mn = 0;
-                    }
-                    if (CH >= 32 || c < CH) {
-                        const uint32_t dst = sb + 16 * c;
-                        const long long ok_ = (long long)mj * a.k.sc_stride_b + (long long)kvh * a.k.sc_stride_h + (long long)mn * NG;
-                        const long long ov_ = (long long)mj * a.v.sc_stride_b + (long long)kvh * a.v.sc_stride_h + (long long)mn * NG;
-                        cp_async16(dst, (const __half*)a.k.scale + ok_, nbytes);
-                        cp_async16(dst + SCB, (const __half*)a.v.scale + ov_, nbytes);
-                        if (ASYM) {
-                            cp_async16(dst + 2 * SCB, (const __half*)a.k.zp + ok_, nbytes);
-                            cp_async16(dst + 3 * SCB, (const __half*)a.v.zp + ov_, nbytes);
-                        }
+                    const int c = c0 + lane, bx = min(c / pieces, nbox - 1), ct = c * 8 / NG;
+                    const int mj = __shfl_sync(0xffffffffu, major, bx);
+                    const int mn = __shfl_sync(0xffffffffu, minor, bx) + ct - bx * box;
+                    // bytes of tokens behind the cache view are not read
+                    const int nbytes = p.pg.table ? 16 : max(0, min(16, (a.max_ctx - mn) * 2 * NG));
+                    if ((CH >= 32 || c < CH) && ((vmask >> bx) & 1) && nbytes) {
+                        const long long off = (long long)mj * cs.sc_stride_b + (long long)kvh * cs.sc_stride_h + (long long)mn * NG;
+                        cp_async16(sb + 16 * c, (const __half*)cs.scale + off, nbytes);
+                        if (ASYM) cp_async16(sb + SCB + 16 * c, (const __half*)cs.zp + off, nbytes);
                     }
                 }
                 cp_async_mbar_arrive(bar);
             }
         };
-        __syncwarp();
-        const int prolog = min(nstage - 1, n_my);
-        for (int k = 0; k < prolog; ++k) issue(k);
+        // this warp is through with part u: the last one to say so fetches the part that takes the slot next
+        auto release = [&](int u) {
+            __syncwarp();
+            uint32_t old = 0;
+            if (lane == 0) old = span_atom_add(done0 + 4 * slot);
+            old = __shfl_sync(0xffffffffu, old, 0);
+            if (old == kSpanWarps - 1) {
+                if (lane == 0) done[slot] = 0;
+                __syncwarp();
+                if (u + kSpanSlots < 2 * ntile) issue(u + kSpanSlots);
+            }
+            if (++slot == kSpanSlots) { slot = 0; phase ^= 1u; }
+        };
+        // A last 128-byte row that a contiguous cache does not fill lies outside the tensor map: its tokens are fetched here
+        // by the warp that they belong to.
+        auto patch = [&](const KvqCacheSide& cs, uint32_t dst, int tok0) {
+            if (TPR == 1 || p.pg.table) return;
+            const int whole = a.max_ctx / TPR * TPR, rest = a.max_ctx - whole, first = tok0 + warp * TSW;
+            if (rest == 0 || whole < first || whole >= first + TSW) return;              // uniform over the warp
+            constexpr int CPT = RB / 16;
+            if (lane < rest * CPT) {
+                const int tk = whole + lane / CPT, c = lane % CPT, row_ = (tk - tok0) / TPR, cc = (tk % TPR) * CPT + c;
+                const uint4 w = *reinterpret_cast<const uint4*>((const char*)cs.payload + (long long)b * cs.pay_stride_b +
+                                                                (long long)kvh * cs.pay_stride_h + (long long)tk * RB + 16 * c);
+                sts128(dst + row_ * 128 + ((cc ^ (row_ & 7)) << 4), w);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");             // before the copy that refills the slot
+            }
+            __syncwarp();
+        };
+        auto wait = [&]() {
+            // after a wait that expired the results are void; the slot protocol goes on to the end, with a short limit, so that
+            // no copy of this CTA is still in flight when it leaves
+            bool ok = false;
+            for (int i = failed ? kWaitLimit - 4096 : 0; i < kWaitLimit && !ok; ++i) ok = mbar_try_wait(bar0 + 8 * slot, phase);
+            if (!__all_sync(0xffffffffu, ok) && !failed) {
+                failed = true;
+                if (lane == 0) atomicOr(&g_span_error_flag, 1);
+            }
+        };
+        if (warp == 0)
+            for (int u = 0; u < min(kSpanSlots, 2 * ntile); ++u) issue(u);
 
         // ---- q fragments: lane (g, t) holds channels of head g in the channel order of the K fragments
         uint32_t qf[NQ];
-        float qb[NG][2];                                       // -offset 2^-24 sum of the group's q, heads 2t and 2t+1
+        float qb[F16 ? 1 : NG][2];                             // -offset 2^-24 sum of the group's q, heads 2t and 2t+1
+        uint32_t qz[2] = {0u, 0u};                             // B fragment of the groups' sums of q: fp16 parts hi, lo
         {
             const bool hv = g < nh;
             const uint32_t* q32 = reinterpret_cast<const uint32_t*>((const __half*)a.q + (long long)b * a.q_stride_b +
@@ -256,20 +300,24 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
             if (!F16) {
 #pragma unroll
                 for (int G = 0; G < NG; ++G) {
-                    float s = qs[G] * (-OFFSET / 16777216.f);
+                    float s = qs[G];
                     s += __shfl_xor_sync(0xffffffffu, s, 1);
-                    s += __shfl_xor_sync(0xffffffffu, s, 2);
-                    qb[G][0] = __shfl_sync(0xffffffffu, s, 8 * t);
-                    qb[G][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);
+                    s += __shfl_xor_sync(0xffffffffu, s, 2);   // sum of q over group G, head g
+                    qb[G][0] = __shfl_sync(0xffffffffu, s, 8 * t) * (-OFFSET * U24);
+                    qb[G][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4) * (-OFFSET * U24);
+                    if (ASYM && (G >> 1) == t) {               // rows 2t, 2t+1 of the B fragment are groups 2t, 2t+1
+                        const __half hi = __float2half_rn(s), lo = __float2half_rn(s - __half2float(hi));
+                        qz[0] |= (uint32_t)__half_as_ushort(hi) << (16 * (G & 1));
+                        qz[1] |= (uint32_t)__half_as_ushort(lo) << (16 * (G & 1));
+                    }
                 }
             }
         }
 
-        float r_run[2] = {-INFINITY, -INFINITY};               // max logit - e, log2 units, heads 2t and 2t+1
-        float m_run[2] = {-INFINITY, -INFINITY};               // max logit
+        float r_run[2] = {-INFINITY, -INFINITY};               // reference of the probabilities, log2 units, heads 2t, 2t+1
         float l_run[2] = {0.f, 0.f};
         float vlim = F16 ? INFINITY : 0.f;                     // largest |scale_v| that the present e allows
-        float e_lift = F16 ? 14.f : 0.f;
+        float e_lift = 12.f;
         float o[D / 16][4];
         float oz[4] = {0.f, 0.f, 0.f, 0.f};                    // rows = groups: sum of P z
 #pragma unroll
@@ -277,220 +325,232 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
 
-        for (int k = 0; k < n_my; ++k) {
-            __syncwarp();                                      // every lane has finished with the slot that is refilled next
-            if (k + nstage - 1 < n_my) issue(k + nstage - 1);
-            const bool ok = mbar_wait_bounded(bar0 + 8 * tslot, tphase);
-            const uint32_t kb = pay_u + tslot * 2 * TILE, vb = kb + TILE;
-            const uint32_t ksb = sc_u + tslot * SCT, vsb = ksb + SCB, kzb = ksb + 2 * SCB, vzb = ksb + 3 * SCB;
-            if (++tslot == nstage) { tslot = 0; tphase ^= 1u; }
-            ++taken;
-            if (!__all_sync(0xffffffffu, ok)) {
-                failed = true;
-                break;
-            }
-            const int tok0 = tile_token<TS>(v, i0 + k * kSpanWarps);
-            const bool partial = !tile_full<TS>(v, tok0);
-            if (TPR > 1 && !p.pg.table) {
-                // a last 128-byte row that the cache does not fill is outside the tensor map: fetch its tokens here
-                const int whole = a.max_ctx / TPR * TPR, rest = a.max_ctx - whole;
-                if (rest && tok0 + TS > whole) {               // uniform over the warp
-                    constexpr int CPT = RB / 16;
-                    if (lane < 2 * rest * CPT) {
-                        const int side = lane >= rest * CPT, x = lane - side * rest * CPT, tk = whole + x / CPT, c = x % CPT;
-                        const KvqCacheSide& cs = side ? a.v : a.k;
-                        const uint4 w = *reinterpret_cast<const uint4*>((const char*)cs.payload + (long long)b * cs.pay_stride_b +
-                                                                        (long long)kvh * cs.pay_stride_h + (long long)tk * RB + 16 * c);
-                        sts128((side ? vb : kb) + span_off<RB, TS>(tk - tok0, c), w);
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // before the copy that refills the slot
-                    }
-                    __syncwarp();
-                }
-            }
+        for (int k = 0; k < ntile; ++k) {
+            const int tok0 = tile_token<TS>(v, cur.i + k), wtok = tok0 + warp * TSW;
+            const bool partial = !tile_full<TSW>(v, wtok);
+            const bool active = wtok < v.n && (wtok + TSW > v.wstart || wtok < v.sinks);       // uniform over the warp
 
             // ================= q.K
             float x[SUB][4];
+            wait();
+            if (active) {
+                const uint32_t kb = ring_u + slot * TILE, ksb = scale_u + slot * SCT + warp * TSW * NG * 2, kzb = ksb + SCB;
+                patch(a.k, kb, tok0);
+                const uint32_t kl = kb + lk;
 #pragma unroll
-            for (int sub = 0; sub < SUB; ++sub) {
-                const int lrow = 16 * sub + ((lane >> 3) & 1) * 8 + (lane & 7);      // ldmatrix row of this lane
-                if (F16) {
+                for (int sub = 0; sub < SUB; ++sub) {
+                    if (F16) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) x[sub][j] = 0.f;
+                        for (int j = 0; j < 4; ++j) x[sub][j] = 0.f;
 #pragma unroll
-                    for (int j = 0; j < D / 16; ++j) {
-                        uint32_t r[4];
-                        ldmatrix_x4(kb + span_off<RB, TS>(lrow, 2 * j + (lane >> 4)), r);
-                        mma16816(x[sub], r[0], r[1], r[2], r[3], qf[2 * j], qf[2 * j + 1]);
-                    }
-                } else {
-                    float s0[NG], s1[NG];                      // scales of token rows g and g + 8
-                    load_row_floats<NG>(ksb + (16 * sub + g) * NG * 2, s0);
-                    load_row_floats<NG>(ksb + (16 * sub + 8 + g) * NG * 2, s1);
-                    float acc[4];
-#pragma unroll
-                    for (int c = 0; c < RB / 16; c += 2) {
-                        uint32_t r[4];
-                        ldmatrix_x4(kb + span_off<RB, TS>(lrow, c + (lane >> 4)), r);
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            constexpr int CPG = I8 ? GS / 16 : GS / 32;        // 16-byte chunks per group
-                            const int cc = c + e, G = cc / CPG;
-                            const uint32_t wa = r[2 * e], wb = r[2 * e + 1];
-                            if (I8) {
-                                const uint32_t ua = wa ^ 0x80808080u, ub = wb ^ 0x80808080u;
-                                const uint32_t a0 = prmt(ua, 0u, 0x4140u), a1 = prmt(ub, 0u, 0x4140u), a2 = prmt(ua, 0u, 0x4342u),
-                                               a3 = prmt(ub, 0u, 0x4342u);
-                                if (cc % CPG == 0) mma16816_from(acc, a0, a1, a2, a3, qf[2 * cc], qf[2 * cc + 1], qb[G][0], qb[G][1]);
-                                else mma16816(acc, a0, a1, a2, a3, qf[2 * cc], qf[2 * cc + 1]);
-                            } else {
-                                const uint32_t wa8 = wa >> 8, wb8 = wb >> 8;
-                                const uint32_t a0 = wa & 0x000F000Fu, a1 = wb & 0x000F000Fu, a2 = wa8 & 0x000F000Fu, a3 = wb8 & 0x000F000Fu;
-                                if (cc % CPG == 0) mma16816_from(acc, a0, a1, a2, a3, qf[4 * cc], qf[4 * cc + 1], qb[G][0], qb[G][1]);
-                                else mma16816(acc, a0, a1, a2, a3, qf[4 * cc], qf[4 * cc + 1]);
-                                mma16816(acc, wa & 0x00F000F0u, wb & 0x00F000F0u, wa8 & 0x00F000F0u, wb8 & 0x00F000F0u, qf[4 * cc + 2],
-                                         qf[4 * cc + 3]);
+                        for (int j = 0; j < D / 16; ++j) {
+                            uint32_t r[4];
+                            ldmatrix_x4(chunk_addr(kl, sub, 2 * j), r);
+                            mma16816(x[sub], r[0], r[1], r[2], r[3], qf[2 * j], qf[2 * j + 1]);
+                        }
+                    } else {
+                        float s0[NG], s1[NG];                  // scales of token rows g and g + 8
+                        load_row_floats<NG>(ksb + (16 * sub + g) * NG * 2, s0);
+                        load_row_floats<NG>(ksb + (16 * sub + 8 + g) * NG * 2, s1);
+                        float xz[4];
+                        if (ASYM) {
+                            // z (16 tokens x groups) times the groups' sums of q: one mma over both fp16 parts of the sums
+                            uint32_t za = 0u, zb = 0u;
+                            if (NG == 1) {
+                                if (t == 0) { za = span_lds16(kzb + (16 * sub + g) * 2); zb = span_lds16(kzb + (16 * sub + 8 + g) * 2); }
+                            } else if (t < NG / 2) {
+                                za = span_lds32(kzb + (16 * sub + g) * NG * 2 + 4 * t);
+                                zb = span_lds32(kzb + (16 * sub + 8 + g) * NG * 2 + 4 * t);
                             }
-                            if (cc % CPG == CPG - 1) {
-                                if (G == 0) {
-                                    x[sub][0] = acc[0] * s0[G]; x[sub][1] = acc[1] * s0[G];
-                                    x[sub][2] = acc[2] * s1[G]; x[sub][3] = acc[3] * s1[G];
+                            mma16816_from(xz, za, zb, za, zb, qz[0], qz[1], 0.f, 0.f);
+                        }
+                        float acc[4];
+#pragma unroll
+                        for (int c = 0; c < RB / 16; c += 2) {
+                            uint32_t r[4];
+                            ldmatrix_x4(chunk_addr(kl, sub, c), r);
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                constexpr int CPG = I8 ? GS / 16 : GS / 32;    // 16-byte chunks per group
+                                const int cc = c + e, G = cc / CPG;
+                                const uint32_t wa = r[2 * e], wb = r[2 * e + 1];
+                                if (I8) {
+                                    const uint32_t ua = wa ^ 0x80808080u, ub = wb ^ 0x80808080u;
+                                    const uint32_t a0 = prmt(ua, 0u, 0x4140u), a1 = prmt(ub, 0u, 0x4140u), a2 = prmt(ua, 0u, 0x4342u),
+                                                   a3 = prmt(ub, 0u, 0x4342u);
+                                    if (cc % CPG == 0) mma16816_from(acc, a0, a1, a2, a3, qf[2 * cc], qf[2 * cc + 1], qb[G][0], qb[G][1]);
+                                    else mma16816(acc, a0, a1, a2, a3, qf[2 * cc], qf[2 * cc + 1]);
                                 } else {
-                                    x[sub][0] = fmaf(acc[0], s0[G], x[sub][0]); x[sub][1] = fmaf(acc[1], s0[G], x[sub][1]);
-                                    x[sub][2] = fmaf(acc[2], s1[G], x[sub][2]); x[sub][3] = fmaf(acc[3], s1[G], x[sub][3]);
+                                    const uint32_t wa8 = wa >> 8, wb8 = wb >> 8;
+                                    const uint32_t a0 = wa & 0x000F000Fu, a1 = wb & 0x000F000Fu, a2 = wa8 & 0x000F000Fu,
+                                                   a3 = wb8 & 0x000F000Fu;
+                                    if (cc % CPG == 0) mma16816_from(acc, a0, a1, a2, a3, qf[4 * cc], qf[4 * cc + 1], qb[G][0], qb[G][1]);
+                                    else mma16816(acc, a0, a1, a2, a3, qf[4 * cc], qf[4 * cc + 1]);
+                                    mma16816(acc, wa & 0x00F000F0u, wb & 0x00F000F0u, wa8 & 0x00F000F0u, wb8 & 0x00F000F0u,
+                                             qf[4 * cc + 2], qf[4 * cc + 3]);
+                                }
+                                if (cc % CPG == CPG - 1) {
+                                    if (G == 0 && !ASYM) {
+                                        x[sub][0] = acc[0] * s0[G]; x[sub][1] = acc[1] * s0[G];
+                                        x[sub][2] = acc[2] * s1[G]; x[sub][3] = acc[3] * s1[G];
+                                    } else if (G == 0) {
+                                        x[sub][0] = fmaf(acc[0], s0[G], xz[0] * U24); x[sub][1] = fmaf(acc[1], s0[G], xz[1] * U24);
+                                        x[sub][2] = fmaf(acc[2], s1[G], xz[2] * U24); x[sub][3] = fmaf(acc[3], s1[G], xz[3] * U24);
+                                    } else {
+                                        x[sub][0] = fmaf(acc[0], s0[G], x[sub][0]); x[sub][1] = fmaf(acc[1], s0[G], x[sub][1]);
+                                        x[sub][2] = fmaf(acc[2], s1[G], x[sub][2]); x[sub][3] = fmaf(acc[3], s1[G], x[sub][3]);
+                                    }
                                 }
                             }
                         }
                     }
-                    if (ASYM) {
-                        load_row_floats<NG>(kzb + (16 * sub + g) * NG * 2, s0);
-                        load_row_floats<NG>(kzb + (16 * sub + 8 + g) * NG * 2, s1);
-#pragma unroll
-                        for (int G = 0; G < NG; ++G) {
-                            const float z0 = s0[G] * (-1.f / OFFSET), z1 = s1[G] * (-1.f / OFFSET);
-                            x[sub][0] = fmaf(z0, qb[G][0], x[sub][0]); x[sub][1] = fmaf(z0, qb[G][1], x[sub][1]);
-                            x[sub][2] = fmaf(z1, qb[G][0], x[sub][2]); x[sub][3] = fmaf(z1, qb[G][1], x[sub][3]);
-                        }
-                    }
                 }
             }
-            if (p.logits) {
-#pragma unroll
-                for (int sub = 0; sub < SUB; ++sub)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int tok = tok0 + 16 * sub + 8 * e + g;
-                        if (tok < v.n)
-                            *reinterpret_cast<float2*>(p.logits + (row * a.max_ctx + tok) * H + 2 * t) =
-                                make_float2(x[sub][2 * e] * scale2, x[sub][2 * e + 1] * scale2);
-                    }
-            }
-            if (partial) {
-#pragma unroll
-                for (int sub = 0; sub < SUB; ++sub) {
-                    const int ta = tok0 + 16 * sub + g;
-                    if (!token_visible(v, ta)) x[sub][0] = x[sub][1] = -INFINITY;
-                    if (!token_visible(v, ta + 8)) x[sub][2] = x[sub][3] = -INFINITY;
-                }
-            }
+            release(2 * k);
 
             // ================= online softmax
-            float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-            for (int sub = 0; sub < SUB; ++sub) {
-                mx[0] = fmaxf(mx[0], fmaxf(x[sub][0], x[sub][2]));
-                mx[1] = fmaxf(mx[1], fmaxf(x[sub][1], x[sub][3]));
-            }
-#pragma unroll
-            for (int off = 4; off <= 16; off <<= 1) {
-                mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], off));
-                mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], off));
-            }
-            if (!F16) {
-                // the largest V scale of the tile: lane = TS * NG / 32 consecutive values
-                constexpr int VPL = TS * NG / 32;              // 1, 2, 4 or 8 fp16 values per lane
-                float vm = 0.f;
-#pragma unroll
-                for (int i = 0; i < VPL; ++i) {
-                    const float s = fabsf(__half2float(__ushort_as_half((unsigned short)span_lds16(vsb + (lane * VPL + i) * 2))));
-                    if (!partial || token_visible(v, tok0 + (lane * VPL + i) / NG)) vm = fmaxf(vm, s);
-                }
-                if (__any_sync(0xffffffffu, vm > vlim)) {
-#pragma unroll
-                    for (int off = 1; off <= 16; off <<= 1) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, off));
-                    // smallest power of two >= vm (frexp: vm = f 2^ex, f in [0.5, 1)); at least 2^-1: 2^e <= 2^15
-                    int ex;
-                    frexpf(fminf(vm, 65504.f), &ex);
-                    ex = max(ex, -1);
-                    vlim = vm > 65504.f ? INFINITY : exp2f((float)ex);
-                    e_lift = 14.f - (float)ex;
-                }
-            }
-            float corr[2], rneg[2];
-            bool changed = false;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                m_run[e] = fmaxf(m_run[e], mx[e] * scale2);
-                const float r_new = m_run[e] == -INFINITY ? -INFINITY : m_run[e] - e_lift;
-                const float ref = r_new == -INFINITY ? 0.f : r_new;      // nothing but -inf so far: p = 0, not NaN
-                changed |= r_new != r_run[e];
-                corr[e] = fast_exp2(r_run[e] - ref);           // exp2(-inf) = 0 on the first tile
-                r_run[e] = r_new;
-                rneg[e] = -ref;
-            }
-            float ps[2] = {0.f, 0.f};
             uint32_t pb[SUB][2];                               // P^T fragments; for NG == 1 with the V scale inside
             uint32_t pz[ASYM && NG == 1 ? SUB : 1][2];         // P^T without the scale, for the zero-points
+            wait();
+            const uint32_t vb = ring_u + slot * TILE, vsb = scale_u + slot * SCT + warp * TSW * NG * 2, vzb = vsb + SCB;
+            if (active) {
+                if (p.logits) {
 #pragma unroll
-            for (int sub = 0; sub < SUB; ++sub) {
-                float p0 = fast_exp2(fmaf(x[sub][0], scale2, rneg[0])), p1 = fast_exp2(fmaf(x[sub][1], scale2, rneg[1]));
-                float p2 = fast_exp2(fmaf(x[sub][2], scale2, rneg[0])), p3 = fast_exp2(fmaf(x[sub][3], scale2, rneg[1]));
-                ps[0] += p0 + p2;
-                ps[1] += p1 + p3;
-                if (!F16 && NG == 1) {
-                    if (ASYM) {
-                        pz[sub][0] = movmatrix_trans(pack_h2(p0, p1));
-                        pz[sub][1] = movmatrix_trans(pack_h2(p2, p3));
-                    }
-                    float va[1], vc[1];
-                    load_row_floats<1>(vsb + (16 * sub + g) * 2, va);
-                    load_row_floats<1>(vsb + (16 * sub + 8 + g) * 2, vc);
-                    if (partial) {                             // slots that are not visible may hold NaN scales
-                        if (!token_visible(v, tok0 + 16 * sub + g)) va[0] = 0.f;
-                        if (!token_visible(v, tok0 + 16 * sub + 8 + g)) vc[0] = 0.f;
-                    }
-                    p0 *= va[0]; p1 *= va[0]; p2 *= vc[0]; p3 *= vc[0];
+                    for (int sub = 0; sub < SUB; ++sub)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int tok = wtok + 16 * sub + 8 * e + g;
+                            if (tok < v.n)
+                                *reinterpret_cast<float2*>(p.logits + (row * a.max_ctx + tok) * H + 2 * t) =
+                                    make_float2(x[sub][2 * e] * scale2, x[sub][2 * e + 1] * scale2);
+                        }
                 }
-                pb[sub][0] = movmatrix_trans(pack_h2(p0, p1));     // tokens 2t, 2t+1 of head g
-                pb[sub][1] = movmatrix_trans(pack_h2(p2, p3));     // tokens 2t+8, 2t+9
-            }
-            l_run[0] = fmaf(l_run[0], corr[0], ps[0]);
-            l_run[1] = fmaf(l_run[1], corr[1], ps[1]);
-            if (__any_sync(0xffffffffu, changed)) {
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
-                    o[i][0] *= corr[0]; o[i][1] *= corr[1]; o[i][2] *= corr[0]; o[i][3] *= corr[1];
-                }
-                if (ASYM) { oz[0] *= corr[0]; oz[1] *= corr[1]; }
-            }
-
-            // ================= P.V
-#pragma unroll
-            for (int sub = 0; sub < SUB; ++sub) {
-                uint32_t mlo = 0xffffffffu, mhi = 0xffffffffu;     // tokens (2t, 2t+1) and (2t+8, 2t+9) that are visible
                 if (partial) {
-                    const int tg = tok0 + 16 * sub + 2 * t;
-                    mlo = (token_visible(v, tg) ? 0x0000ffffu : 0u) | (token_visible(v, tg + 1) ? 0xffff0000u : 0u);
-                    mhi = (token_visible(v, tg + 8) ? 0x0000ffffu : 0u) | (token_visible(v, tg + 9) ? 0xffff0000u : 0u);
-                }
-                if (F16) {
-                    const int vrow = 16 * sub + (lane >> 4) * 8 + (lane & 7);
 #pragma unroll
-                    for (int i = 0; i < D / 16; ++i) {
-                        uint32_t r[4];
-                        ldmatrix_x4_trans(vb + span_off<RB, TS>(vrow, 2 * i + ((lane >> 3) & 1)), r);
-                        mma16816(o[i], r[0] & mlo, r[1] & mlo, r[2] & mhi, r[3] & mhi, pb[sub][0], pb[sub][1]);
+                    for (int sub = 0; sub < SUB; ++sub) {
+                        const int ta = wtok + 16 * sub + g;
+                        if (!token_visible(v, ta)) x[sub][0] = x[sub][1] = -INFINITY;
+                        if (!token_visible(v, ta + 8)) x[sub][2] = x[sub][3] = -INFINITY;
                     }
-                } else {
+                }
+                float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int sub = 0; sub < SUB; ++sub) {
+                    mx[0] = fmaxf(mx[0], fmaxf(x[sub][0], x[sub][2]));
+                    mx[1] = fmaxf(mx[1], fmaxf(x[sub][1], x[sub][3]));
+                }
+                float r_new[2] = {r_run[0], r_run[1]};
+                bool moved = false;
+                if (!F16) {
+                    // the largest V scale of the share: TSW * NG / 32 consecutive values per lane
+                    constexpr int VPL = TSW * NG / 32;         // 1, 2, 4 or 8
+                    float vm = 0.f;
+                    if (!partial && VPL >= 2) {
+                        __half2 m2 = u32_as_h2(span_lds32(vsb + lane * VPL * 2) & 0x7fff7fffu);
+#pragma unroll
+                        for (int i = 1; i < VPL / 2; ++i) m2 = __hmax2(m2, u32_as_h2(span_lds32(vsb + lane * VPL * 2 + 4 * i) & 0x7fff7fffu));
+                        const float2 f = __half22float2(m2);
+                        vm = fmaxf(f.x, f.y);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < VPL; ++i) {
+                            const float s = fabsf(__half2float(__ushort_as_half((unsigned short)span_lds16(vsb + (lane * VPL + i) * 2))));
+                            if (!partial || token_visible(v, wtok + (lane * VPL + i) / NG)) vm = fmaxf(vm, s);
+                        }
+                    }
+                    if (__any_sync(0xffffffffu, vm > vlim)) {
+#pragma unroll
+                        for (int off = 1; off <= 16; off <<= 1) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, off));
+                        // the power of two above vm (frexp: vm = f 2^ex, f in [0.5, 1)); at least 1: 2^(e + 3) <= 2^15
+                        int ex;
+                        frexpf(fminf(vm, 65504.f), &ex);
+                        ex = max(ex, 0);
+                        vlim = vm > 65504.f ? INFINITY : exp2f((float)ex);
+                        const float e_new = 12.f - (float)ex;
+                        r_new[0] += e_lift - e_new;            // e only falls: P shrinks with it
+                        r_new[1] += e_lift - e_new;
+                        e_lift = e_new;
+                        moved = true;
+                    }
+                }
+                // P stays below 2^(e + 3): the reference moves only when a logit rises that far above the maximum that set it
+                // (-inf - -inf = NaN compares false: nothing but -inf so far)
+                const float over = fmaxf(mx[0] * scale2 - r_new[0], mx[1] * scale2 - r_new[1]);
+                if (__any_sync(0xffffffffu, over > e_lift + 3.f)) {
+#pragma unroll
+                    for (int off = 4; off <= 16; off <<= 1) {
+                        mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], off));
+                        mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], off));
+                    }
+                    r_new[0] = fmaxf(r_new[0], mx[0] * scale2 - e_lift);
+                    r_new[1] = fmaxf(r_new[1], mx[1] * scale2 - e_lift);
+                    moved = true;
+                }
+                if (moved) {                                   // uniform over the warp
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        // exp2(-inf) = 0 the first time; a reference that stays -inf has nothing to scale
+                        const float c = r_new[e] == r_run[e] ? 1.f : fast_exp2(r_run[e] - r_new[e]);
+                        l_run[e] *= c;
+#pragma unroll
+                        for (int i = 0; i < D / 16; ++i) {
+                            o[i][e] *= c;
+                            o[i][2 + e] *= c;
+                        }
+                        if (ASYM) oz[e] *= c;
+                        r_run[e] = r_new[e];
+                    }
+                }
+                const float rneg[2] = {r_run[0] == -INFINITY ? 0.f : -r_run[0], r_run[1] == -INFINITY ? 0.f : -r_run[1]};
+                float ps[2] = {0.f, 0.f};
+#pragma unroll
+                for (int sub = 0; sub < SUB; ++sub) {
+                    float p0 = fast_exp2(fmaf(x[sub][0], scale2, rneg[0])), p1 = fast_exp2(fmaf(x[sub][1], scale2, rneg[1]));
+                    float p2 = fast_exp2(fmaf(x[sub][2], scale2, rneg[0])), p3 = fast_exp2(fmaf(x[sub][3], scale2, rneg[1]));
+                    ps[0] += p0 + p2;
+                    ps[1] += p1 + p3;
+                    if (!F16 && NG == 1) {
+                        if (ASYM) {
+                            pz[sub][0] = movmatrix_trans(pack_h2(p0, p1));
+                            pz[sub][1] = movmatrix_trans(pack_h2(p2, p3));
+                        }
+                        float va[1], vc[1];
+                        load_row_floats<1>(vsb + (16 * sub + g) * 2, va);
+                        load_row_floats<1>(vsb + (16 * sub + 8 + g) * 2, vc);
+                        if (partial) {                         // slots that are not visible may hold NaN scales
+                            if (!token_visible(v, wtok + 16 * sub + g)) va[0] = 0.f;
+                            if (!token_visible(v, wtok + 16 * sub + 8 + g)) vc[0] = 0.f;
+                        }
+                        p0 *= va[0]; p1 *= va[0]; p2 *= vc[0]; p3 *= vc[0];
+                    }
+                    pb[sub][0] = movmatrix_trans(pack_h2(p0, p1));     // tokens 2t, 2t+1 of head g
+                    pb[sub][1] = movmatrix_trans(pack_h2(p2, p3));     // tokens 2t+8, 2t+9
+                }
+                l_run[0] += ps[0];
+                l_run[1] += ps[1];
+
+                // ================= P.V
+                patch(a.v, vb, tok0);
+                const uint32_t vl = vb + lv;
+                float sp[NG][4];                               // sum of P scale_v over the tile, per group: heads 2t, 2t+1
+#pragma unroll
+                for (int sub = 0; sub < SUB; ++sub) {
+                    uint32_t mlo = 0xffffffffu, mhi = 0xffffffffu;     // tokens (2t, 2t+1) and (2t+8, 2t+9) that are visible
+                    if (partial) {
+                        const int tg = wtok + 16 * sub + 2 * t;
+                        mlo = (token_visible(v, tg) ? 0x0000ffffu : 0u) | (token_visible(v, tg + 1) ? 0xffff0000u : 0u);
+                        mhi = (token_visible(v, tg + 8) ? 0x0000ffffu : 0u) | (token_visible(v, tg + 9) ? 0xffff0000u : 0u);
+                    }
+                    if (F16) {
+#pragma unroll
+                        for (int i = 0; i < D / 16; ++i) {
+                            uint32_t r[4];
+                            ldmatrix_x4_trans(chunk_addr(vl, sub, 2 * i), r);
+                            if (partial) { r[0] &= mlo; r[1] &= mlo; r[2] &= mhi; r[3] &= mhi; }
+                            mma16816(o[i], r[0], r[1], r[2], r[3], pb[sub][0], pb[sub][1]);
+                        }
+                        continue;
+                    }
                     uint32_t pg[NG][2];
                     if (NG == 1) {
                         pg[0][0] = pb[sub][0];
@@ -505,6 +565,12 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
                             pg[G][1] = hmul2_u(pb[sub][1], sy[G]);
                         }
                     }
+                    constexpr uint32_t kOnes = 0x3c003c00u;
+#pragma unroll
+                    for (int G = 0; G < NG; ++G) {
+                        if (sub == 0) mma16816_from(sp[G], kOnes, kOnes, kOnes, kOnes, pg[G][0], pg[G][1], 0.f, 0.f);
+                        else mma16816(sp[G], kOnes, kOnes, kOnes, kOnes, pg[G][0], pg[G][1]);
+                    }
                     if (ASYM) {
                         uint32_t zlo = 0u, zhi = 0u;           // row g = group g: (z[2t], z[2t+1]), (z[2t+8], z[2t+9])
                         if (g < NG) {
@@ -512,42 +578,47 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
                             zlo = (span_lds16(za) | (span_lds16(za + 2 * NG) << 16)) & mlo;
                             zhi = (span_lds16(za + 16 * NG) | (span_lds16(za + 18 * NG) << 16)) & mhi;
                         }
-                        mma16816(oz, zlo, 0u, zhi, 0u, NG == 1 ? pz[ASYM && NG == 1 ? sub : 0][0] : pb[sub][0],
-                                 NG == 1 ? pz[ASYM && NG == 1 ? sub : 0][1] : pb[sub][1]);
+                        const int zs = ASYM && NG == 1 ? sub : 0;
+                        mma16816(oz, zlo, 0u, zhi, 0u, NG == 1 ? pz[zs][0] : pb[sub][0], NG == 1 ? pz[zs][1] : pb[sub][1]);
                     }
-                    const int lrow = 16 * sub + ((lane >> 3) & 1) * 8 + (lane & 7);
 #pragma unroll
                     for (int c = 0; c < RB / 16; c += 2) {
                         uint32_t r[4];
-                        ldmatrix_x4_trans(vb + span_off<RB, TS>(lrow, c + (lane >> 4)), r);
+                        ldmatrix_x4_trans(chunk_addr(vl, sub, c), r);
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
                             const int cc = c + e;
                             if (I8) {
                                 const uint32_t X = r[2 * e] ^ 0x80808080u, Y = r[2 * e + 1] ^ 0x80808080u;
                                 const int G = 16 * cc / GS;
-                                mma16816(o[cc], i8pair_to_h2(X, 0x5240u), i8pair_to_h2(X, 0x5341u), i8pair_to_h2(Y, 0x5240u),
-                                         i8pair_to_h2(Y, 0x5341u), pg[G][0], pg[G][1]);
+                                mma16816(o[cc], prmt(X, 0u, 0x4240u), prmt(X, 0u, 0x4341u), prmt(Y, 0u, 0x4240u), prmt(Y, 0u, 0x4341u),
+                                         pg[G][0], pg[G][1]);
                             } else {
                                 const uint32_t X = r[2 * e], Y = r[2 * e + 1], X8 = X >> 8, Y8 = Y >> 8;
                                 const int G = 32 * cc / GS;
-                                mma16816(o[2 * cc], nib_hi_to_h2(X), nib_lo_to_h2(X), nib_hi_to_h2(Y), nib_lo_to_h2(Y), pg[G][0], pg[G][1]);
-                                mma16816(o[2 * cc + 1], nib_hi_to_h2(X8), nib_lo_to_h2(X8), nib_hi_to_h2(Y8), nib_lo_to_h2(Y8), pg[G][0],
+                                mma16816(o[2 * cc], X & 0x00F000F0u, X & 0x000F000Fu, Y & 0x00F000F0u, Y & 0x000F000Fu, pg[G][0], pg[G][1]);
+                                mma16816(o[2 * cc + 1], X8 & 0x00F000F0u, X8 & 0x000F000Fu, Y8 & 0x00F000F0u, Y8 & 0x000F000Fu, pg[G][0],
                                          pg[G][1]);
                             }
                         }
                     }
                 }
+                if (!F16) {
+                    // take the codes' offset out again, tile by tile: what is cancelled is never more than one tile's worth
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        const int G = 16 * i / GS;
+                        const float c0 = I8 ? OFFSET * U24 : 16.f * OFFSET * U24, c1 = OFFSET * U24;   // high nibbles count 16-fold
+                        o[i][0] = fmaf(sp[G][0], -c0, o[i][0]); o[i][1] = fmaf(sp[G][1], -c0, o[i][1]);
+                        o[i][2] = fmaf(sp[G][0], -c1, o[i][2]); o[i][3] = fmaf(sp[G][1], -c1, o[i][3]);
+                    }
+                }
             }
-        }
-        if (failed) {                                          // give the other copies in flight a chance to land
-            if (lane == 0) atomicOr(&g_span_error_flag, 1);
-            for (; taken < issued; ++taken) {
-                mbar_wait_bounded(bar0 + 8 * tslot, tphase);
-                if (++tslot == nstage) { tslot = 0; tphase ^= 1u; }
-            }
+            release(2 * k + 1);
         }
 
+        cur.left -= ntile;
+        if (cur.left <= 0) pdl_launch_dependents();            // the join may be set up; it waits for this kernel's end
         // ---- merge the warps through the ring's memory (every copy of this row has landed), leave the partial or the output
 #pragma unroll
         for (int off = 4; off <= 16; off <<= 1) {
@@ -566,16 +637,17 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
             ra[(2 * t) * DR + D + g] = oz[0];
             ra[(2 * t + 1) * DR + D + g] = oz[1];
         }
+        constexpr float f0 = F16 ? 1.f : I8 ? 1.f / U24 : 1.f / (16.f * U24), f1 = F16 ? 1.f : 1.f / U24;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
             int d0, d1;                                        // channels of fragment rows g and g + 8
             if (F16) { d0 = 16 * i + g; d1 = d0 + 8; }
             else if (I8) { d0 = 16 * i + 2 * g; d1 = d0 + 1; }
             else { d0 = 32 * (i >> 1) + 4 * g + 2 * (i & 1); d1 = d0 + 1; }
-            ra[(2 * t) * DR + d0] = o[i][0];
-            ra[(2 * t + 1) * DR + d0] = o[i][1];
-            ra[(2 * t) * DR + d1] = o[i][2];
-            ra[(2 * t + 1) * DR + d1] = o[i][3];
+            ra[(2 * t) * DR + d0] = o[i][0] * f0;
+            ra[(2 * t + 1) * DR + d0] = o[i][1] * f0;
+            ra[(2 * t) * DR + d1] = o[i][2] * f1;
+            ra[(2 * t + 1) * DR + d1] = o[i][3] * f1;
         }
         __syncthreads();
         if (threadIdx.x < H) {
@@ -622,7 +694,6 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
                 if (d == 0) { p.ws_ml[(slot * H + h) * 2] = M; p.ws_ml[(slot * H + h) * 2 + 1] = L; }
             }
         }
-        cur.left -= i1 - cur.i;
         if (cur.left <= 0) break;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();                                       // the ring may be written again
