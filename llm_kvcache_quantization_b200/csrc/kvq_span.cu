@@ -200,12 +200,15 @@ static int span_plan(const KvqSpanAttnArgs& s, SpanPlan& pl) {
     });
     pl.rows = (long long)a.B * p.hr;
     const long long per_row = max_visible_tiles(p, pl.ts);
-    if (pl.rows * per_row >= (1LL << 31) || pl.rows >= (1LL << 30) || a.B > 65535) return KVQ_ELIMIT;
-    // A warp of the generic kernel takes a whole tile, so a run has at least 4; the tensor-core kernel's tiles are the CTA's.
-    // A row of at most 256 tokens is not worth cutting: it takes one CTA, and the join is saved.
-    p.min_tiles = pl.kind ? 1 : 4;
+    if (pl.rows * (per_row + 64) >= (1LL << 31) || pl.rows >= (1LL << 30) || a.B > 65535) return KVQ_ELIMIT;
+    // A row of at most 256 tokens is not worth cutting (no join: INT8 1 x 2 heads of 304 slots 11.9 -> 8.1 us at 200 tokens).
+    // Otherwise a CTA has at least one tile (the generic kernel: one for each warp), and the cut counts the work of starting
+    // a row (q, lookups, writing the part) as one more tile, on long rows only: of short ones it would leave CTAs idle.
+    // INT8 32 x 8 K, 148 x 3 CTAs: 60.4 us without it, 57.8 with; INT4 with zero-points 1 x 1.2 K tokens 11.4 without, 13.4.
     p.row_mode = per_row * pl.ts <= 256;
-    long long ctas = (pl.rows * per_row + p.min_tiles - 1) / p.min_tiles;
+    p.row_cost = p.row_mode ? 0 : pl.kind ? (per_row >= 16 ? 1 : 0) : 4;
+    p.min_tiles = (pl.kind ? 1 : 4) + p.row_cost;
+    long long ctas = (pl.rows * (per_row + p.row_cost) + p.min_tiles - 1) / p.min_tiles;
     p.ctas = p.row_mode ? (int)pl.rows : (int)(ctas < slots ? ctas : slots);
     const size_t parts = p.row_mode ? 0 : (size_t)p.ctas + pl.rows;
     pl.o_bytes = pad256(parts * kHeadsPerCta * a.D * sizeof(float));

@@ -6,11 +6,13 @@
 //
 // Cut.  A row (batch row b, kv head, chunk of 8 query heads) is a list of token tiles of TS tokens: the tiles that the
 // sinks touch, then the tiles from the window's first token to the last token.  The tiles of all rows, laid end to end,
-// are divided into equal runs, one per CTA of a single resident wave; a CTA walks its run and leaves one unnormalised
+// with a few imaginary ones in front of each row for what it costs to start and to end it, are divided into runs whose lengths
+// differ by at most one, one per CTA of a single resident wave; a CTA walks the tiles of its run and leaves one unnormalised
 // partial (o, m, l) per row that it met.  The partial of (CTA c, row r) has slot c + r: along the runs either c or r grows
 // from one partial to the next, so slots are distinct and at most ctas + rows of them exist.  The join recomputes the cut
 // and finds the CTAs of its row.  With one run per row (`row_mode`, short spans) the kernel writes the output itself and
-// there is no join.
+// there is no join.  (Measured and not kept: the CTA that arrives last at a row joins it - atomics on one word by up to 74
+// CTAs and one CTA reading all partials cost more than a second launch, 33 us against 19 for a window of 4 K tokens x 32 rows.)
 #pragma once
 
 #include <cuda_fp16.h>
@@ -28,7 +30,8 @@ struct SpanParams {
     int n_rep, rep_chunks;
     int hr;                 // rows per batch row: Hkv * rep_chunks
     int ctas;               // runs the tiles are cut into
-    int min_tiles;          // a run has at least this many tiles
+    int min_tiles;          // a run has at least this many units
+    int row_cost;           // imaginary tiles in front of a row
     int row_mode;           // one run per row, direct output
     float* ws_o;            // [ctas + rows][8][D]
     float* ws_ml;           // [ctas + rows][8][2]   (m in log2 units, l)
@@ -73,85 +76,91 @@ __device__ __forceinline__ bool tile_full(const RowView& v, int tok0) {
     return tok0 + TS <= v.n && (tok0 >= v.wstart || tok0 + TS <= v.sinks);
 }
 
-// The run of CTA `cta`: `left` tiles from tile `i` of row (b, hr).  Called by every thread; NT threads, `sh` >= NT / 32 + 4 ints.
+// The cut: runs 0 .. longer-1 have q + 1 tiles, the others q.
+struct SpanCut {
+    int runs, q, longer;
+};
+__device__ __forceinline__ SpanCut span_cut(const SpanParams& p, int total) {
+    SpanCut k;
+    k.runs = max(1, min(p.ctas, (int)((unsigned)total / (unsigned)p.min_tiles)));
+    k.q = (unsigned)total / (unsigned)k.runs;
+    k.longer = total - k.q * k.runs;
+    return k;
+}
+__device__ __forceinline__ int span_first(const SpanCut& k, int c) { return c * k.q + min(c, k.longer); }
+__device__ __forceinline__ int span_run_of(const SpanCut& k, int u) {          // the run of tile u
+    const int edge = k.longer * (k.q + 1);
+    return u < edge ? (unsigned)u / (unsigned)(k.q + 1) : k.longer + (int)((unsigned)(u - edge) / (unsigned)k.q);
+}
+
+// The run of CTA `cta`: `left` units (imaginary and real tiles) from unit `i` of row (b, hr); unit row_cost is the row's
+// first tile.  Every warp finds it by itself: no barrier.
 struct SpanCursor {
     int b, hr, i, left;
+    int u;                  // the run's next unit in the count over all rows
+    SpanCut cut;
 };
-template <int TS, int NT>
-__device__ __forceinline__ SpanCursor span_locate(const SpanParams& p, int cta, int* sh) {
+template <int TS>
+__device__ __forceinline__ int row_units(const SpanParams& p, int b) {
+    const int t = row_view<TS>(p, b).tiles;
+    return t > 0 ? t + p.row_cost : 0;
+}
+template <int TS>
+__device__ __forceinline__ SpanCursor span_locate(const SpanParams& p, int cta) {
     SpanCursor c;
+    c.b = c.hr = c.i = c.left = c.u = 0;
+    c.cut.runs = c.cut.q = c.cut.longer = 0;
     if (p.row_mode) {
         c.b = cta / p.hr;
         c.hr = cta - c.b * p.hr;
-        c.i = 0;
-        c.left = row_view<TS>(p, c.b).tiles;
+        c.left = row_units<TS>(p, c.b);
         return c;
     }
-    constexpr int NW = NT / 32;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (p.a.B == 1) {
-        const int tiles = row_view<TS>(p, 0).tiles, total = tiles * p.hr;
-        const int per = max((total + p.ctas - 1) / p.ctas, p.min_tiles);
-        const long long u0 = (long long)cta * per;
-        c.b = 0;
-        c.left = u0 < total ? min(per, total - (int)u0) : 0;
-        c.hr = c.left ? (int)u0 / tiles : 0;
-        c.i = c.left ? (int)u0 - c.hr * tiles : 0;
-        return c;
-    }
-    // sum of the rows' tiles, then the row whose tiles contain the first one of the run
-    int mine = 0;
-    for (int b = tid; b < p.a.B; b += NT) mine += row_view<TS>(p, b).tiles;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    if (lane == 0) sh[warp] = mine;
-    __syncthreads();
+    const int lane = threadIdx.x & 31;
     int sum = 0;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) sum += sh[w];
+#pragma unroll 1
+    for (int b = lane; b < p.a.B; b += 32) sum += row_units<TS>(p, b);
+    sum = __reduce_add_sync(0xffffffffu, sum);
     const int total = sum * p.hr;
-    const int per = max((total + p.ctas - 1) / p.ctas, p.min_tiles);
-    const long long u0l = (long long)cta * per;
-    if (u0l >= total) {                                    // uniform over the CTA
-        c.b = c.hr = c.i = c.left = 0;
-        return c;
-    }
-    const int u0 = (int)u0l;
-    c.left = min(per, total - u0);
-    int before = 0;
-    for (int b0 = 0; b0 < p.a.B; b0 += NT) {
-        const int t = b0 + tid < p.a.B ? row_view<TS>(p, b0 + tid).tiles : 0;
+    if (total == 0) return c;
+    c.cut = span_cut(p, total);
+    if (cta >= c.cut.runs) return c;
+    c.u = span_first(c.cut, cta);
+    c.left = span_first(c.cut, cta + 1) - c.u;
+    int before = 0;                                        // units of the batch rows in front of this group of 32
+#pragma unroll 1
+    for (int b0 = 0;; b0 += 32) {
+        const int t = b0 + lane < p.a.B ? row_units<TS>(p, b0 + lane) * p.hr : 0;
         int incl = t;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int x = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += x;
         }
-        __syncthreads();                                   // sh is free again
-        if (lane == 31) sh[warp] = incl;
-        __syncthreads();
-        int all = 0;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            if (w < warp) incl += sh[w];
-            all += sh[w];
+        const unsigned past = __ballot_sync(0xffffffffu, c.u < before + incl);
+        if (past) {                                        // the first lane whose rows reach beyond unit u
+            const int l = __ffs(past) - 1;
+            const int off = c.u - before - __shfl_sync(0xffffffffu, incl - t, l);
+            const int units = __shfl_sync(0xffffffffu, t, l) / p.hr;
+            c.b = b0 + l;
+            c.hr = off / units;
+            c.i = off - c.hr * units;
+            return c;
         }
-        const int lo = (before + incl - t) * p.hr, hi = (before + incl) * p.hr;
-        if (u0 >= lo && u0 < hi) {
-            sh[NW] = b0 + tid;
-            sh[NW + 1] = u0 - lo;
-            sh[NW + 2] = t;
-        }
-        before += all;
-        if (u0 < before * p.hr) break;                     // uniform
+        before += __shfl_sync(0xffffffffu, incl, 31);
     }
-    __syncthreads();
-    c.b = sh[NW];
-    const int off = sh[NW + 1], tiles = sh[NW + 2];
-    c.hr = off / tiles;
-    c.i = off - c.hr * tiles;
-    __syncthreads();
-    return c;
+}
+// Tiles [i0, i1) of the row of a cursor that belong to the run, and the units that it takes
+struct SpanPiece {
+    int i0, i1, units;
+};
+__device__ __forceinline__ SpanPiece span_piece(const SpanParams& p, const SpanCursor& c, const RowView& v) {
+    SpanPiece s;
+    const int end = min(v.tiles > 0 ? v.tiles + p.row_cost : 0, c.i + c.left);
+    s.units = end - c.i;
+    s.i0 = max(c.i - p.row_cost, 0);
+    s.i1 = max(end - p.row_cost, 0);
+    return s;
 }
 // Next row of a run (a row's tiles are used up): skips rows without tiles.
 template <int TS>
@@ -227,10 +236,9 @@ __global__ void __launch_bounds__(128) span_generic_kernel(const SpanParams p) {
     const int gs = a.group_size;
     __shared__ float q_s[H][D];
     __shared__ float red_ml[NW][H][2];
-    __shared__ int sh[NW + 4];
     extern __shared__ float red_acc[];                     // [NW][H][D]
     pdl_wait();
-    SpanCursor c = span_locate<TS, 128>(p, blockIdx.x, sh);
+    SpanCursor c = span_locate<TS>(p, blockIdx.x);
     if (c.left == 0 && !p.row_mode) return;
     const float qk_scale = a.sm_scale * kLog2e;
     RowView v = row_view<TS>(p, c.b);
@@ -238,7 +246,8 @@ __global__ void __launch_bounds__(128) span_generic_kernel(const SpanParams p) {
         const int b = c.b, kvh = c.hr / p.rep_chunks, rc = c.hr - kvh * p.rep_chunks;
         const int h0 = kvh * p.n_rep + rc * H, nh = min(H, p.n_rep - rc * H);
         const int row = b * p.hr + c.hr;
-        const int i1 = min(v.tiles, c.i + c.left);
+        const SpanPiece pc = span_piece(p, c, v);
+        if (pc.i0 < pc.i1 || p.row_mode) {                 // not only imaginary ones; uniform over the CTA
         __syncthreads();
         for (int i = tid; i < H * D; i += 128) {
             const int h = i / D, d = i % D;
@@ -259,7 +268,7 @@ __global__ void __launch_bounds__(128) span_generic_kernel(const SpanParams p) {
 #pragma unroll
             for (int e = 0; e < EPL; ++e) acc[h][e] = 0.f;
         }
-        for (int i = c.i + warp; i < i1; i += NW) {
+        for (int i = pc.i0 + warp; i < pc.i1; i += NW) {
             const int tok0 = tile_token<TS>(v, i), tok = tok0 + lane;
             const bool valid = token_visible(v, tok);
             float s[H];
@@ -363,7 +372,9 @@ __global__ void __launch_bounds__(128) span_generic_kernel(const SpanParams p) {
                 if (d == 0) { p.ws_ml[(slot * H + h) * 2] = M; p.ws_ml[(slot * H + h) * 2 + 1] = L; }
             }
         }
-        c.left -= i1 - c.i;
+        }
+        c.left -= pc.units;
+        c.u += pc.units;
         if (c.left <= 0) break;                            // uniform
         span_next_row<TS>(p, c, v);
     }
@@ -379,34 +390,32 @@ template <int EPL, int TS>
 __global__ void __launch_bounds__(kJoinThreads) span_join_kernel(const SpanParams p) {
     constexpr int D = EPL * 32, H = kHeadsPerCta, NW = kJoinThreads / 32, U = 4;
     pdl_launch_dependents();
-    pdl_wait();
     const KvqAttnArgs& a = p.a;
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    __shared__ int shs[NW][2];
     __shared__ float red[NW][D + 1];
     __shared__ float red_m[NW];
+    // The cut, before the wait for the partials: this kernel starts only when every CTA of the one before is past its own
+    // wait, so the lengths are there.
     const int tiles = row_view<TS>(p, b).tiles;
     int sum = 0, before = 0;
-    for (int i = tid; i < a.B; i += kJoinThreads) {
-        const int t = row_view<TS>(p, i).tiles;
+#pragma unroll 1
+    for (int i = lane; i < a.B; i += 32) {
+        const int t = row_units<TS>(p, i);
         sum += t;
         if (i < b) before += t;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        before += __shfl_xor_sync(0xffffffffu, before, o);
-    }
-    if (lane == 0) { shs[warp][0] = sum; shs[warp][1] = before; }
-    __syncthreads();
-    sum = before = 0;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) { sum += shs[w][0]; before += shs[w][1]; }
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    before = __reduce_add_sync(0xffffffffu, before);
     const int kvh = h / p.n_rep, hk = h - kvh * p.n_rep, rc = hk / H, hl = hk - rc * H;
     const int hr = kvh * p.rep_chunks + rc, row = b * p.hr + hr;
-    const int total = sum * p.hr, per = max((total + p.ctas - 1) / p.ctas, p.min_tiles);
-    const int u0 = before * p.hr + hr * tiles;
-    const int c0 = u0 / per, c1 = tiles > 0 ? (u0 + tiles - 1) / per : c0 - 1;
+    int c0 = 0, c1 = -1;
+    if (tiles > 0) {
+        const SpanCut cut = span_cut(p, sum * p.hr);
+        const int first = before * p.hr + hr * (tiles + p.row_cost) + p.row_cost;
+        c0 = span_run_of(cut, first);
+        c1 = span_run_of(cut, first + tiles - 1);
+    }
+    pdl_wait();
 
     float M = -INFINITY, L = 0.f, acc[EPL];
 #pragma unroll

@@ -16,12 +16,14 @@
 // Both roundings of P are relative as long as P scale_v stays in fp16's normal range, whatever the scales: probabilities are
 // 2^(x - r) with r = (a maximum of the logits x so far) - e, where e keeps 2^(e+3) scale_v <= 2^15 for the largest scale met
 // so far, and r moves only when a logit exceeds it by e + 3: no maximum over the warp in most tiles.
-// Copies.  A CTA walks tiles of 4 x TSW tokens, TSW per warp, so that the K or the V part of a tile is 16 KB; the parts
-// take turns in a ring of 3 slots (4 CTAs of 4 warps fit an SM).  One warp fetches a part for all: payload by
-// cp.async.bulk.tensor (128-byte rows, 128-byte swizzle; rows shorter than that hold 2 or 4 tokens, longer ones come as 2
-// halves), one copy per page piece or warp share that has a visible token, scales by 16-byte cp.async, all on the slot's
-// mbarrier.  The warp that finishes a slot last refills it, so there is no producer warp and no barrier inside a row.  Waits
-// are bounded; an expired one raises bit 0 of the error flag.
+// Copies.  A CTA walks tiles of 4 x TSW tokens, TSW per warp, through a ring of slots that each hold the K, the V and the
+// scales of a tile.  One warp fetches a tile for all: payload by cp.async.bulk.tensor (128-byte rows, 128-byte swizzle; rows
+// shorter than that hold 2 or 4 tokens, longer ones come as 2 halves), scales by cp.async.bulk, one copy per page piece or
+// warp share that has a visible token, all on the slot's mbarrier.  The warp that finishes a slot last refills it, so there
+// is no producer warp and no barrier inside a row; every warp has looked up the pages of the tile that the slot takes next by
+// then.  Waits are bounded; an expired one raises bit 0 of the error flag.
+// (Measured and not kept, INT8 32 x 8 K / INT4 16 x 8 K, 60 / 28 us before: K and V parts in slots of their own 60 / 28, with
+// 8 KB slots 64 / 36; a ring per warp 62 / 35.)
 #pragma once
 
 #include "kvq_ptx.cuh"
@@ -30,21 +32,23 @@
 namespace kvq {
 
 constexpr int kSpanWarps = 4;
-constexpr int kSpanSlots = 3;
+constexpr int kSpanMaxSlots = 4;
 
 template <int FMT, bool ASYM, int GS, int D>
 struct SpanShape {
     static constexpr bool F16 = FMT == KVQ_FMT_FP16;
     static constexpr int RB = F16 ? 2 * D : FMT == KVQ_FMT_INT8 ? D : D / 2;   // payload bytes of a token
     static constexpr int TPR = RB < 128 ? 128 / RB : 1;                        // tokens per 128-byte row
-    static constexpr int TSW = RB >= 256 ? 16 : RB == 128 ? 32 : 64;           // tokens of a warp
+    static constexpr int TSW = RB >= 256 ? 16 : RB >= 64 ? 32 : 64;            // tokens of a warp
     static constexpr int TS = kSpanWarps * TSW;                                // tokens of a tile
     static constexpr int NG = F16 ? 1 : D / GS;
-    static constexpr int TILE = TS * RB;                                       // bytes of K (or V) of a tile: a ring slot
+    static constexpr int TILE = TS * RB;                                       // bytes of K (or V) of a tile
     static constexpr int SCB = F16 ? 0 : TS * NG * 2;                          // bytes of one scale table of a tile
-    static constexpr int SCT = (ASYM ? 2 : 1) * SCB;
+    static constexpr int SCT = (ASYM ? 2 : 1) * SCB;                           // scales (and zero-points) of K, or of V
+    static constexpr int SLOT = 2 * TILE;                                      // payload of a slot; the scales of all slots follow
+    static constexpr int SLOTS = 2;
     static constexpr size_t smem() {
-        const size_t ring = (size_t)kSpanSlots * (TILE + SCT);
+        const size_t ring = (size_t)SLOTS * (SLOT + 2 * SCT);
         const size_t red = (size_t)kSpanWarps * kHeadsPerCta * (D + 8) * 4;
         return (ring > red ? ring : red) + 1024;
     }
@@ -58,6 +62,15 @@ struct SpanMmaParams {
 __device__ __forceinline__ void sts128(uint32_t addr, uint4 v) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
+__device__ __forceinline__ void sts16(uint32_t addr, unsigned short v) {
+    asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(v) : "memory");
+}
+// `bytes` (a multiple of 16) from 16-byte aligned global memory, counted on the barrier
+__device__ __forceinline__ void span_bulk(uint32_t dst, const void* src, int bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
 __device__ __forceinline__ uint32_t span_lds32(uint32_t addr) {
     uint32_t w;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(addr));
@@ -89,7 +102,7 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
     using S = SpanShape<FMT, ASYM, GS, D>;
     constexpr bool F16 = S::F16, I8 = FMT == KVQ_FMT_INT8;
     constexpr int RB = S::RB, TPR = S::TPR, TS = S::TS, TSW = S::TSW, NG = S::NG, TILE = S::TILE, SCB = S::SCB, SCT = S::SCT;
-    constexpr int SUB = TSW / 16, H = kHeadsPerCta;
+    constexpr int SUB = TSW / 16, H = kHeadsPerCta, SLOT = S::SLOT, SLOTS = S::SLOTS;
     constexpr int NQ = D / 8;                                  // fragment registers of q
     constexpr int SUBSTEP = 16 * (RB < 128 ? RB : 128);        // bytes between 16-token pieces of a tile
     constexpr float OFFSET = I8 ? 128.f : 8.f;
@@ -101,18 +114,17 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
 
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* smem = smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u);
-    const uint32_t ring_u = smem_u32(smem), scale_u = ring_u + kSpanSlots * TILE;
-    __shared__ __align__(8) unsigned long long bars[kSpanSlots];
-    __shared__ uint32_t done[kSpanSlots];                      // warps that have finished with a slot
+    const uint32_t ring_u = smem_u32(smem), scale_u = ring_u + SLOTS * SLOT;
+    __shared__ __align__(8) unsigned long long bars[SLOTS];
+    __shared__ uint32_t done[SLOTS];                      // warps that have finished with a slot
     __shared__ float red_ml[kSpanWarps][H][2];
     __shared__ float red_w[kSpanWarps][H];
     __shared__ float red_tot[H][2];
-    __shared__ int sh[kSpanWarps + 4];
 
     const uint32_t bar0 = smem_u32(&bars[0]), done0 = smem_u32(&done[0]);
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kSpanSlots; ++s) {
-            mbar_init(bar0 + 8 * s, F16 ? 1 : 33);             // expect_tx (+ 32 cp.async arrivals)
+        for (int s = 0; s < SLOTS; ++s) {
+            mbar_init(bar0 + 8 * s, 1);
             done[s] = 0;
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -123,7 +135,7 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
     __syncthreads();
     pdl_wait();                                                // q, the cache, the lengths and the table
 
-    SpanCursor cur = span_locate<TS, kSpanWarps * 32>(p, blockIdx.x, sh);
+    SpanCursor cur = span_locate<TS>(p, blockIdx.x);
     if (cur.left == 0 && !p.row_mode) return;                  // uniform over the CTA
     RowView v = row_view<TS>(p, cur.b);
     const float scale2 = fabsf(a.sm_scale) * kLog2e * (F16 ? 1.f : 1.f / U24);       // q carries the sign; subnormal codes
@@ -145,6 +157,9 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
         if (RB == 32 && (sub & 1)) x ^= 64u;                   // four tokens a row: the swizzle's row number moves by 4
         return x + sub * SUBSTEP + (RB > 128 ? (c >> 3) * (TS * 128) : 0);
     };
+    // where the cache view ends, if the copies leave something of its last tokens out
+    constexpr int PER = TPR > 8 / NG ? TPR : 8 / NG;           // tokens that fill a row and 16 bytes of scales
+    const int tail = F16 || p.pg.table || a.max_ctx % PER == 0 ? -1 : a.max_ctx;
     int slot = 0;
     uint32_t phase = 0;
     bool failed = false;
@@ -153,84 +168,98 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
         const int b = cur.b, kvh = cur.hr / p.rep_chunks, rc = cur.hr - kvh * p.rep_chunks;
         const int h0 = kvh * p.n_rep + rc * H, nh = min(H, p.n_rep - rc * H);
         const long long row = (long long)b * p.hr + cur.hr;
-        const int i1 = min(v.tiles, cur.i + cur.left), ntile = i1 - cur.i;
-        const int slot0 = slot;                                // slot of part 0 of this row
+        const SpanPiece pc = span_piece(p, cur, v);            // tiles i0 .. i1 - 1 of the row are this run's
+        if (pc.i0 < pc.i1 || p.row_mode) {                     // not only imaginary ones
+        const int ntile = pc.i1 - pc.i0;
+        const int slot0 = slot;                                // slot of the row's first tile
 
-        // ---- request part u (K of tile u / 2 for even u, V for odd u) into its slot; called by one whole warp
-        auto issue = [&](int u) {
-            const int side = u & 1, tok0 = tile_token<TS>(v, cur.i + (u >> 1));
-            const int s = (slot0 + u) % kSpanSlots;
-            const uint32_t dst = ring_u + s * TILE, sb = scale_u + s * SCT, bar = bar0 + 8 * s;
-            const KvqCacheSide& cs = side ? a.v : a.k;
-            // batch row or page, and the row in it, of the piece of `box` tokens that this lane's number names
-            const int tok = tok0 + lane * box;
-            const bool vis = lane < nbox && tok < v.n && (tok + box > v.wstart || tok < v.sinks);
-            int major = b, minor = tok;
+        // Where piece `lane` (of `box` tokens) of tile k is: batch row or page, and the row in it
+        int major, minor;
+        bool vis;                                              // it has a visible token
+        auto place = [&](int k) {
+            const int tok = tile_token<TS>(v, pc.i0 + k) + lane * box;
+            vis = k < ntile && lane < nbox && tok < v.n && (tok + box > v.wstart || tok < v.sinks);
+            major = b;
+            minor = tok;
             if (p.pg.table && vis) {
                 const int blk = tok / p.pg.page_size;
                 major = __ldg(p.pg.table + b * p.pg.stride_b + blk);
                 minor = tok - blk * p.pg.page_size;
-                if (major < 0 || major >= p.pg.num_pages) {
+            }
+        };
+        // ---- request the tile that place() looked up into slot s; called by one whole warp
+        auto issue = [&](int s) {
+            const uint32_t dst = ring_u + s * SLOT, sb = scale_u + s * 2 * SCT, bar = bar0 + 8 * s;
+            // scales of the piece; the last token row of a contiguous cache may end inside 16 bytes, see patch()
+            int sbytes = 0, all = 0;
+            if (vis) {
+                if (p.pg.table && (major < 0 || major >= p.pg.num_pages)) {
                     atomicOr(&g_span_error_flag, 2);
                     major = 0;
                 }
+                if (!F16) sbytes = min(box, p.pg.table ? box : a.max_ctx - minor) * (2 * NG) & ~15;
+                all = 2 * box * RB + (ASYM ? 4 : 2) * sbytes;
             }
-            const unsigned vmask = __ballot_sync(0xffffffffu, vis);
-            if (lane == 0) mbar_expect_tx(bar, __popc(vmask) * box * RB);
+            all = __reduce_add_sync(0xffffffffu, all);
+            if (lane == 0) mbar_expect_tx(bar, all);
             __syncwarp();
             if (vis) {
-                const CUtensorMap* map = side ? &vmap : &kmap;
                 const uint32_t d = dst + lane * box * (RB < 128 ? RB : 128);
-                tma_load_4d(d, map, bar, 0, minor / TPR, kvh, major);
-                if (RB > 128) tma_load_4d(d + TS * 128, map, bar, 128, minor / TPR, kvh, major);
-            }
-            if (!F16) {
-                constexpr int CH = TS * NG / 8;                // 16-byte chunks of one scale table
-                const int pieces = box * NG / 8;               // of them in a piece
-#pragma unroll
-                for (int c0 = 0; c0 < CH; c0 += 32) {
-                    const int c = c0 + lane, bx = min(c / pieces, nbox - 1), ct = c * 8 / NG;
-                    const int mj = __shfl_sync(0xffffffffu, major, bx);
-                    const int mn = __shfl_sync(0xffffffffu, minor, bx) + ct - bx * box;
-                    // bytes of tokens behind the cache view are not read
-                    const int nbytes = p.pg.table ? 16 : max(0, min(16, (a.max_ctx - mn) * 2 * NG));
-                    if ((CH >= 32 || c < CH) && ((vmask >> bx) & 1) && nbytes) {
-                        const long long off = (long long)mj * cs.sc_stride_b + (long long)kvh * cs.sc_stride_h + (long long)mn * NG;
-                        cp_async16(sb + 16 * c, (const __half*)cs.scale + off, nbytes);
-                        if (ASYM) cp_async16(sb + SCB + 16 * c, (const __half*)cs.zp + off, nbytes);
+                tma_load_4d(d, &kmap, bar, 0, minor / TPR, kvh, major);
+                if (RB > 128) tma_load_4d(d + TS * 128, &kmap, bar, 128, minor / TPR, kvh, major);
+                tma_load_4d(d + TILE, &vmap, bar, 0, minor / TPR, kvh, major);
+                if (RB > 128) tma_load_4d(d + TILE + TS * 128, &vmap, bar, 128, minor / TPR, kvh, major);
+                if (!F16 && sbytes) {
+                    const uint32_t ds = sb + lane * box * (2 * NG);
+                    const long long ok_ = (long long)major * a.k.sc_stride_b + (long long)kvh * a.k.sc_stride_h + minor * NG;
+                    const long long ov_ = (long long)major * a.v.sc_stride_b + (long long)kvh * a.v.sc_stride_h + minor * NG;
+                    span_bulk(ds, (const __half*)a.k.scale + ok_, sbytes, bar);
+                    span_bulk(ds + SCT, (const __half*)a.v.scale + ov_, sbytes, bar);
+                    if (ASYM) {
+                        span_bulk(ds + SCB, (const __half*)a.k.zp + ok_, sbytes, bar);
+                        span_bulk(ds + SCT + SCB, (const __half*)a.v.zp + ov_, sbytes, bar);
                     }
                 }
-                cp_async_mbar_arrive(bar);
             }
         };
-        // this warp is through with part u: the last one to say so fetches the part that takes the slot next
-        auto release = [&](int u) {
-            __syncwarp();
-            uint32_t old = 0;
-            if (lane == 0) old = span_atom_add(done0 + 4 * slot);
-            old = __shfl_sync(0xffffffffu, old, 0);
-            if (old == kSpanWarps - 1) {
-                if (lane == 0) done[slot] = 0;
-                __syncwarp();
-                if (u + kSpanSlots < 2 * ntile) issue(u + kSpanSlots);
-            }
-            if (++slot == kSpanSlots) { slot = 0; phase ^= 1u; }
-        };
-        // A last 128-byte row that a contiguous cache does not fill lies outside the tensor map: its tokens are fetched here
-        // by the warp that they belong to.
-        auto patch = [&](const KvqCacheSide& cs, uint32_t dst, int tok0) {
-            if (TPR == 1 || p.pg.table) return;
-            const int whole = a.max_ctx / TPR * TPR, rest = a.max_ctx - whole, first = tok0 + warp * TSW;
-            if (rest == 0 || whole < first || whole >= first + TSW) return;              // uniform over the warp
+        // What the copies leave out at the end of a contiguous cache, fetched with plain loads by the warp that owns the tokens:
+        // a last 128-byte row that the cache does not fill (it lies outside the tensor map) and scales that do not fill 16 bytes.
+        auto patch = [&](const KvqCacheSide& cs, uint32_t dst, uint32_t sdst, int tok0) {
+            const int whole = a.max_ctx / TPR * TPR, rest = a.max_ctx - whole;
             constexpr int CPT = RB / 16;
             if (lane < rest * CPT) {
                 const int tk = whole + lane / CPT, c = lane % CPT, row_ = (tk - tok0) / TPR, cc = (tk % TPR) * CPT + c;
                 const uint4 w = *reinterpret_cast<const uint4*>((const char*)cs.payload + (long long)b * cs.pay_stride_b +
                                                                 (long long)kvh * cs.pay_stride_h + (long long)tk * RB + 16 * c);
                 sts128(dst + row_ * 128 + ((cc ^ (row_ & 7)) << 4), w);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");             // before the copy that refills the slot
             }
-            __syncwarp();
+            const int swhole = a.max_ctx * NG & ~7, srest = a.max_ctx * NG - swhole;          // fp16 values
+            if (lane < srest) {
+                const long long off = (long long)b * cs.sc_stride_b + (long long)kvh * cs.sc_stride_h + swhole + lane;
+                const uint32_t d = sdst + (swhole - tok0 * NG + lane) * 2;
+                sts16(d, ((const unsigned short*)cs.scale)[off]);
+                if (ASYM) sts16(d + SCB, ((const unsigned short*)cs.zp)[off]);
+            }
+        };
+        // Tokens of the warp's share that are not visible may hold anything, NaN included.  Their logits become -inf, so P is
+        // 0; what P is multiplied with is overwritten with zeros here (fp16: the V rows, else the V scales and zero-points).
+        auto blank = [&](uint32_t vb, uint32_t vsb, int wtok) {
+#pragma unroll 1
+            for (int r = lane; r < TSW; r += 32) {
+                if (token_visible(v, wtok + r)) continue;
+                if (F16) {
+                    const int rr = warp * TSW + r;
+#pragma unroll 1
+                    for (int c = 0; c < RB / 16; ++c)
+                        sts128(vb + (c >> 3) * (TS * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), make_uint4(0u, 0u, 0u, 0u));
+                } else {
+#pragma unroll 1
+                    for (int j = 0; j < NG; ++j) {
+                        sts16(vsb + (r * NG + j) * 2, 0);
+                        if (ASYM) sts16(vsb + SCB + (r * NG + j) * 2, 0);
+                    }
+                }
+            }
         };
         auto wait = [&]() {
             // after a wait that expired the results are void; the slot protocol goes on to the end, with a short limit, so that
@@ -242,8 +271,13 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
                 if (lane == 0) atomicOr(&g_span_error_flag, 1);
             }
         };
-        if (warp == 0)
-            for (int u = 0; u < min(kSpanSlots, 2 * ntile); ++u) issue(u);
+        if (warp == 0) {
+#pragma unroll 1
+            for (int k = 0; k < min(SLOTS, ntile); ++k) {
+                place(k);
+                issue((slot0 + k) % SLOTS);
+            }
+        }
 
         // ---- q fragments: lane (g, t) holds channels of head g in the channel order of the K fragments
         uint32_t qf[NQ];
@@ -326,16 +360,26 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
             for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
 
         for (int k = 0; k < ntile; ++k) {
-            const int tok0 = tile_token<TS>(v, cur.i + k), wtok = tok0 + warp * TSW;
-            const bool partial = !tile_full<TSW>(v, wtok);
+            if (p.pg.table) place(k + SLOTS);                  // the tile that takes this slot next
+            const int tok0 = tile_token<TS>(v, pc.i0 + k), wtok = tok0 + warp * TSW;
+            const bool partial = !tile_full<TSW>(v, wtok) || (tail > wtok && tail <= wtok + TSW);
             const bool active = wtok < v.n && (wtok + TSW > v.wstart || wtok < v.sinks);       // uniform over the warp
 
             // ================= q.K
             float x[SUB][4];
             wait();
             if (active) {
-                const uint32_t kb = ring_u + slot * TILE, ksb = scale_u + slot * SCT + warp * TSW * NG * 2, kzb = ksb + SCB;
-                patch(a.k, kb, tok0);
+                const uint32_t kb = ring_u + slot * SLOT, ksb = scale_u + slot * 2 * SCT + warp * TSW * NG * 2, kzb = ksb + SCB;
+                if (partial) {
+                    if (tail > wtok && tail <= wtok + TSW) {
+                        patch(a.k, kb, scale_u + slot * 2 * SCT, tok0);
+                        patch(a.v, kb + TILE, scale_u + slot * 2 * SCT + SCT, tok0);
+                        __syncwarp();
+                    }
+                    blank(kb + TILE, ksb + SCT, wtok);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // before the copy that refills the slot
+                    __syncwarp();
+                }
                 const uint32_t kl = kb + lk;
 #pragma unroll
                 for (int sub = 0; sub < SUB; ++sub) {
@@ -406,13 +450,10 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
                     }
                 }
             }
-            release(2 * k);
-
             // ================= online softmax
             uint32_t pb[SUB][2];                               // P^T fragments; for NG == 1 with the V scale inside
             uint32_t pz[ASYM && NG == 1 ? SUB : 1][2];         // P^T without the scale, for the zero-points
-            wait();
-            const uint32_t vb = ring_u + slot * TILE, vsb = scale_u + slot * SCT + warp * TSW * NG * 2, vzb = vsb + SCB;
+            const uint32_t vb = ring_u + slot * SLOT + TILE, vsb = scale_u + slot * 2 * SCT + SCT + warp * TSW * NG * 2, vzb = vsb + SCB;
             if (active) {
                 if (p.logits) {
 #pragma unroll
@@ -445,7 +486,7 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
                     // the largest V scale of the share: TSW * NG / 32 consecutive values per lane
                     constexpr int VPL = TSW * NG / 32;         // 1, 2, 4 or 8
                     float vm = 0.f;
-                    if (!partial && VPL >= 2) {
+                    if (VPL >= 2) {
                         __half2 m2 = u32_as_h2(span_lds32(vsb + lane * VPL * 2) & 0x7fff7fffu);
 #pragma unroll
                         for (int i = 1; i < VPL / 2; ++i) m2 = __hmax2(m2, u32_as_h2(span_lds32(vsb + lane * VPL * 2 + 4 * i) & 0x7fff7fffu));
@@ -455,17 +496,15 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
 #pragma unroll
                         for (int i = 0; i < VPL; ++i) {
                             const float s = fabsf(__half2float(__ushort_as_half((unsigned short)span_lds16(vsb + (lane * VPL + i) * 2))));
-                            if (!partial || token_visible(v, wtok + (lane * VPL + i) / NG)) vm = fmaxf(vm, s);
+                            vm = fmaxf(vm, s);
                         }
                     }
                     if (__any_sync(0xffffffffu, vm > vlim)) {
 #pragma unroll
                         for (int off = 1; off <= 16; off <<= 1) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, off));
-                        // the power of two above vm (frexp: vm = f 2^ex, f in [0.5, 1)); at least 1: 2^(e + 3) <= 2^15
-                        int ex;
-                        frexpf(fminf(vm, 65504.f), &ex);
-                        ex = max(ex, 0);
-                        vlim = vm > 65504.f ? INFINITY : exp2f((float)ex);
+                        // exponent of the power of two above vm; at least 0: 2^(e + 3) <= 2^15
+                        const int ex = max((int)(__float_as_uint(fminf(vm, 65504.f)) >> 23) - 126, 0);
+                        vlim = vm > 65504.f ? INFINITY : __uint_as_float((uint32_t)(ex + 127) << 23);
                         const float e_new = 12.f - (float)ex;
                         r_new[0] += e_lift - e_new;            // e only falls: P shrinks with it
                         r_new[1] += e_lift - e_new;
@@ -517,10 +556,6 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
                         float va[1], vc[1];
                         load_row_floats<1>(vsb + (16 * sub + g) * 2, va);
                         load_row_floats<1>(vsb + (16 * sub + 8 + g) * 2, vc);
-                        if (partial) {                         // slots that are not visible may hold NaN scales
-                            if (!token_visible(v, wtok + 16 * sub + g)) va[0] = 0.f;
-                            if (!token_visible(v, wtok + 16 * sub + 8 + g)) vc[0] = 0.f;
-                        }
                         p0 *= va[0]; p1 *= va[0]; p2 *= vc[0]; p3 *= vc[0];
                     }
                     pb[sub][0] = movmatrix_trans(pack_h2(p0, p1));     // tokens 2t, 2t+1 of head g
@@ -530,23 +565,15 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
                 l_run[1] += ps[1];
 
                 // ================= P.V
-                patch(a.v, vb, tok0);
                 const uint32_t vl = vb + lv;
                 float sp[NG][4];                               // sum of P scale_v over the tile, per group: heads 2t, 2t+1
 #pragma unroll
                 for (int sub = 0; sub < SUB; ++sub) {
-                    uint32_t mlo = 0xffffffffu, mhi = 0xffffffffu;     // tokens (2t, 2t+1) and (2t+8, 2t+9) that are visible
-                    if (partial) {
-                        const int tg = wtok + 16 * sub + 2 * t;
-                        mlo = (token_visible(v, tg) ? 0x0000ffffu : 0u) | (token_visible(v, tg + 1) ? 0xffff0000u : 0u);
-                        mhi = (token_visible(v, tg + 8) ? 0x0000ffffu : 0u) | (token_visible(v, tg + 9) ? 0xffff0000u : 0u);
-                    }
                     if (F16) {
 #pragma unroll
                         for (int i = 0; i < D / 16; ++i) {
                             uint32_t r[4];
                             ldmatrix_x4_trans(chunk_addr(vl, sub, 2 * i), r);
-                            if (partial) { r[0] &= mlo; r[1] &= mlo; r[2] &= mhi; r[3] &= mhi; }
                             mma16816(o[i], r[0], r[1], r[2], r[3], pb[sub][0], pb[sub][1]);
                         }
                         continue;
@@ -557,8 +584,8 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
                         pg[0][1] = pb[sub][1];
                     } else {
                         uint32_t sx[NG], sy[NG];
-                        load_scale_pairs<NG>(vsb + (16 * sub + 2 * t) * 2 * NG, sx, mlo);
-                        load_scale_pairs<NG>(vsb + (16 * sub + 2 * t + 8) * 2 * NG, sy, mhi);
+                        load_scale_pairs<NG>(vsb + (16 * sub + 2 * t) * 2 * NG, sx, 0xffffffffu);
+                        load_scale_pairs<NG>(vsb + (16 * sub + 2 * t + 8) * 2 * NG, sy, 0xffffffffu);
 #pragma unroll
                         for (int G = 0; G < NG; ++G) {
                             pg[G][0] = hmul2_u(pb[sub][0], sx[G]);
@@ -575,8 +602,8 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
                         uint32_t zlo = 0u, zhi = 0u;           // row g = group g: (z[2t], z[2t+1]), (z[2t+8], z[2t+9])
                         if (g < NG) {
                             const uint32_t za = vzb + ((16 * sub + 2 * t) * NG + g) * 2;
-                            zlo = (span_lds16(za) | (span_lds16(za + 2 * NG) << 16)) & mlo;
-                            zhi = (span_lds16(za + 16 * NG) | (span_lds16(za + 18 * NG) << 16)) & mhi;
+                            zlo = span_lds16(za) | (span_lds16(za + 2 * NG) << 16);
+                            zhi = span_lds16(za + 16 * NG) | (span_lds16(za + 18 * NG) << 16);
                         }
                         const int zs = ASYM && NG == 1 ? sub : 0;
                         mma16816(oz, zlo, 0u, zhi, 0u, NG == 1 ? pz[zs][0] : pb[sub][0], NG == 1 ? pz[zs][1] : pb[sub][1]);
@@ -614,11 +641,23 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
                     }
                 }
             }
-            release(2 * k + 1);
+            // through with the slot: the last warp to say so fetches the tile that takes it next
+            __syncwarp();
+            uint32_t old = 0;
+            if (lane == 0) old = span_atom_add(done0 + 4 * slot);
+            old = __shfl_sync(0xffffffffu, old, 0);
+            if (old == kSpanWarps - 1) {
+                if (lane == 0) done[slot] = 0;
+                __syncwarp();
+                if (k + SLOTS < ntile) {
+                    if (!p.pg.table) place(k + SLOTS);
+                    issue(slot);
+                }
+            }
+            if (++slot == SLOTS) { slot = 0; phase ^= 1u; }
         }
 
-        cur.left -= ntile;
-        if (cur.left <= 0) pdl_launch_dependents();            // the join may be set up; it waits for this kernel's end
+        if (cur.left <= pc.units) pdl_launch_dependents();     // the join may be set up; it waits for this kernel's end
         // ---- merge the warps through the ring's memory (every copy of this row has landed), leave the partial or the output
 #pragma unroll
         for (int off = 4; off <= 16; off <<= 1) {
@@ -694,6 +733,9 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
                 if (d == 0) { p.ws_ml[(slot * H + h) * 2] = M; p.ws_ml[(slot * H + h) * 2 + 1] = L; }
             }
         }
+        }
+        cur.left -= pc.units;
+        cur.u += pc.units;
         if (cur.left <= 0) break;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();                                       // the ring may be written again
