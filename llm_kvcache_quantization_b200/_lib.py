@@ -223,6 +223,7 @@ STRUCTS = (KvqAppendSide, KvqAppendArgs, KvqCacheSide, KvqAttnArgs, KvqCombineAr
            KvqPagedReadArgs, KvqEvictBuf, KvqEvictArgs)
 
 _LIB = None
+_MARSHAL = None
 
 
 class KvqError(RuntimeError):
@@ -262,6 +263,27 @@ def load():
                               f"{C.sizeof(st)} in the binding")
     _LIB = lib
     return lib
+
+
+def marshal():
+    """The module that marshals the calls of the bounded- and paged-cache entry points, bound to `load()`'s library."""
+    global _MARSHAL
+    if _MARSHAL is None:
+        lib = load()
+        try:
+            from . import _marshal
+        except ImportError as e:
+            raise ImportError(f"{_build.MARSHAL_PATH}: {e}. Build it with `python -m llm_kvcache_quantization_b200.build` "
+                              "for this interpreter and this torch") from e
+        for name, which in (("SPAN_ATTN", 11), ("PAGED_APPEND", 12), ("PAGED_READ", 13), ("EVICT", 15)):
+            if getattr(_marshal, name) != lib.kvq_struct_size(which):
+                raise ImportError(f"{_build.MARSHAL_PATH} was built for other argument structs than {lib_path()}: "
+                                  "rebuild it with `python -m llm_kvcache_quantization_b200.build --force`")
+        _marshal.bind(check, *(C.cast(getattr(lib, f), C.c_void_p).value for f in (
+            "kvq_span_attn", "kvq_span_attn_workspace_bytes", "kvq_paged_append", "kvq_paged_read", "kvq_evict",
+            "kvq_evict_workspace_bytes")))
+        _MARSHAL = _marshal
+    return _MARSHAL
 
 
 def check(fn: str, code: int) -> None:

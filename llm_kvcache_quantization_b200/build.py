@@ -1,4 +1,5 @@
-"""Builds libkvq.so (the C-ABI CUDA library) in-tree with nvcc for sm_100a.
+"""Builds libkvq.so (the C-ABI CUDA library) in-tree with nvcc for sm_100a, and _marshal.so (the host-side argument
+marshalling of some of its entry points, a Python module against torch's headers) with the C++ compiler.
 
     python -m llm_kvcache_quantization_b200.build [--force] [--verbose] [-DNAME=VALUE ...] [--out PATH]
 
@@ -13,11 +14,14 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
 INCLUDE = os.path.join(os.path.dirname(PKG_DIR), "include")
 LIB_PATH = os.path.join(PKG_DIR, "libkvq.so")
+MARSHAL_SOURCE = os.path.join(CSRC, "kvq_marshal.cpp")
+MARSHAL_PATH = os.path.join(PKG_DIR, "_marshal.so")
 
 SOURCES = ("kvq_api.cu", "kvq_quantize.cu", "kvq_decode.cu", "kvq_dequantize.cu", "kvq_calibrate.cu", "kvq_kivi.cu",
            "kvq_span.cu", "kvq_paged.cu", "kvq_evict.cu")
@@ -43,8 +47,28 @@ def _stale() -> bool:
     if not os.path.exists(LIB_PATH):
         return True
     t = os.path.getmtime(LIB_PATH)
-    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [os.path.join(INCLUDE, "kvq.h"), __file__]
+    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if not f.endswith(".cpp")] + [os.path.join(INCLUDE, "kvq.h"), __file__]
     return any(os.path.getmtime(d) > t for d in deps)
+
+
+def _build_marshal(force: bool, verbose: bool) -> None:
+    deps = (MARSHAL_SOURCE, os.path.join(INCLUDE, "kvq.h"), __file__)
+    if not force and os.path.exists(MARSHAL_PATH) and \
+            all(os.path.getmtime(d) <= os.path.getmtime(MARSHAL_PATH) for d in deps):
+        return
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", INCLUDE,
+           "-I", os.path.join(root, "include"), "-I", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           "-I", sysconfig.get_paths()["include"], "-I", os.path.join(cuda, "include"), MARSHAL_SOURCE,
+           "-o", MARSHAL_PATH, "-L", os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if verbose or proc.returncode != 0:
+        sys.stderr.write(proc.stdout + proc.stderr)
+    if proc.returncode != 0:
+        raise RuntimeError("the C++ compiler failed building _marshal.so")
 
 
 def build(force: bool = False, verbose: bool = False, defines=(), out: str | None = None) -> str:
@@ -53,6 +77,8 @@ def build(force: bool = False, verbose: bool = False, defines=(), out: str | Non
     if out is None and defines:
         raise ValueError("a build with extra defines needs its own output path")
     target = out or LIB_PATH
+    if out is None:
+        _build_marshal(force, verbose)
     if out is None and not force and not _stale():
         return LIB_PATH
     cmd = [_nvcc(), "-shared", "-o", target, "-I", INCLUDE, "-I", CSRC, *NVCC_FLAGS]

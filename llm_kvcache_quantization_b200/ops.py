@@ -642,6 +642,17 @@ def _page_table(table: torch.Tensor, batch: int, pool: torch.Tensor) -> _lib.Kvq
     return _lib.KvqPageTable(table.data_ptr(), table.stride(0), table.shape[1], pool.shape[2], pool.shape[0])
 
 
+_MARSHAL = None
+
+
+def _marshal():
+    """_marshal.so takes the ordinary calls of the functions below; it returns None, with nothing done, for any other, and
+    the function then goes on in Python, where every check, conversion and message is."""
+    global _MARSHAL
+    _MARSHAL = _lib.marshal()
+    return _MARSHAL
+
+
 def span_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor],
               v_scale: Optional[torch.Tensor], context_lens: Optional[torch.Tensor], sm_scale: Optional[float] = None, *,
               k_zp=None, v_zp=None, block_table: Optional[torch.Tensor] = None, window: Optional[int] = None, sinks: int = 0,
@@ -649,6 +660,10 @@ def span_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: Option
               inv_tau: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """q_len == 1 attention over the visible span of a contiguous cache [B, Hkv, S, .] or, with `block_table`, of page
     pools [num_pages, Hkv, page_size, .] (`kvq_span_attn`).  No host synchronisation: lengths are clamped on the device."""
+    done = (_MARSHAL or _marshal()).span_attn(q, k, v, k_scale, v_scale, context_lens, sm_scale, k_zp, v_zp, block_table,
+                                              window, sinks, weights, max_ctx, inv_tau, out)
+    if done is not None:
+        return done
     dev = _require_cuda(q, k, v, k_scale, v_scale, k_zp, v_zp, context_lens, block_table, weights, inv_tau, out)
     if q.ndim != 3:
         raise ValueError(f"q must have shape [B, Hq, D], got {tuple(q.shape)}")
@@ -674,6 +689,8 @@ def span_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: Option
         if k.shape[0] != B:
             raise ValueError(f"Batch mismatch: q={B}, k={k.shape[0]}")
         span = k.shape[2]
+        if span >= 2 ** 31:
+            raise ValueError(f"a cache holds less than 2^31 slots, got {span}")
     else:
         s.pages = _page_table(block_table, B, k)
         span = min(block_table.shape[1] * k.shape[2], 2 ** 31 - 1)
@@ -730,6 +747,9 @@ def paged_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pages: torch.Tensor
     """Quantize new tokens [B, Hkv, T, D] into pages, one launch (`kvq_paged_append`): token t of row b goes to position
     start_pos[b] + t of the row, t < new_lens[b] (default: all).  Scales: min / max with zero-points when zero-point pools
     are given, the static tables [Hkv, G] when those are given, else the `clip_percentile` of each group's magnitudes."""
+    if (_MARSHAL or _marshal()).paged_append(k_new, v_new, k_pages, v_pages, k_scale, v_scale, block_table, start_pos, new_lens,
+                                             k_zp, v_zp, k_static, v_static, clip_percentile):
+        return
     dev = _require_cuda(k_new, v_new, k_pages, v_pages, k_scale, v_scale, k_zp, v_zp, block_table, start_pos, new_lens,
                         k_static, v_static)
     if k_new.ndim != 4 or k_new.shape != v_new.shape:
@@ -781,6 +801,10 @@ def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: Optional[t
     """Tokens start_pos[b] + t (default start 0), t < lens[b] (default `tokens`), of every row as fp16 (k, v)
     [B, Hkv, tokens, head_dim]; zeros behind lens[b] (`kvq_paged_read`).  Values are code * scale (+ zero-point), rounded
     once.  `head_dim` tells nibble-packed pages (width head_dim / 2) from INT8 ones."""
+    done = (_MARSHAL or _marshal()).paged_read(k_pages, v_pages, k_scale, v_scale, block_table, start_pos, tokens, lens,
+                                               head_dim, k_zp, v_zp)
+    if done is not None:
+        return done
     dev = _require_cuda(k_pages, v_pages, k_scale, v_scale, k_zp, v_zp, block_table, start_pos, lens)
     D, T = int(head_dim), int(tokens)
     if D not in (64, 128, 256):
@@ -818,6 +842,9 @@ def evict(weights: torch.Tensor, positions: torch.Tensor, lengths: torch.Tensor,
     """Shrink every (batch row, kv head) of a contiguous cache to `budget` tokens, in place (`kvq_evict`); returns the new
     lengths, int32 [B]."""
     buffers = tuple(buffers)
+    done = (_MARSHAL or _marshal()).evict(weights, positions, lengths, seen, budget, buffers, sinks, recent)
+    if done is not None:
+        return done
     dev = _require_cuda(weights, positions, lengths, seen, *buffers)
     if weights.dtype != torch.float32 or weights.ndim != 3:
         raise ValueError(f"weights must be fp32 [B, Hkv, slots], got {weights.dtype} {tuple(weights.shape)}")
