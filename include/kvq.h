@@ -495,7 +495,7 @@ KVQ_API int kvq_paged_read(const KvqPagedReadArgs* args, kvq_stream_t stream);
  *   Kept tokens in slots < budget stay.  The i-th kept token behind them (slots ascending) moves to the i-th freed slot:
  *   its row of every buffer, its weight, its position.  Afterwards positions of slots < budget are >= 0, positions of
  *   slots budget..n_b-1 are -1 and their weights 0; buffer rows behind the budget and all slots >= n_b are left as they were.
- *   new_lengths[b] = min(n_b, budget) (may alias lengths).  Rows with n_b <= budget are left as they were.
+ *   new_lengths[b] = min(n_b, budget) (not the array `lengths`).  Rows with n_b <= budget are left as they were.
  * Keys carry their rotary position, so their order in the cache does not matter to kvq_decode_attn.
  */
 #define KVQ_EVICT_MAX_BUFS 10

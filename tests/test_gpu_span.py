@@ -437,6 +437,40 @@ def test_evict(case, kind):
     assert torch.equal(ld.cpu(), lens) and torch.equal(sd.cpu(), seen)
 
 
+@pytest.mark.parametrize("kind", ("random", "ties", "equal", "special"))
+@pytest.mark.parametrize("cap,n,budget", ((4096, 4096, 2000), (4097, 4097, 4000), (32768, 32768, 300), (32769, 32769, 30000),
+                                          (70000, 69999, 20000)))
+def test_evict_long_rows(cap, n, budget, kind):
+    """Runs of one slot more or less than a CTA's, runs that are read again by every pass, large and small shares."""
+    gen = torch.Generator().manual_seed(cap)
+    EVICT.append((1, 1, cap, [n], budget, 4, 64, 0))
+    try:
+        w, pos, lens, seen = _evict_inputs(len(EVICT) - 1, kind, gen)
+    finally:
+        EVICT.pop()
+    k = torch.arange(cap, dtype=torch.int32).view(1, 1, cap, 1)
+    rw, rp, rn, moves = evict(w, pos, lens, seen, budget, 4, 64)
+    wd, pd, ld, sd, kd = _d(w, pos, lens, seen, k)
+    got = kvq.evict_tokens(wd, pd, ld, sd, budget, [kd], sinks=4, recent=64)
+    dst, src = moves[0, 0]
+    k[0, 0, dst, 0] = torch.tensor(src, dtype=torch.int32)
+    assert torch.equal(got.cpu(), rn) and torch.equal(pd.cpu(), rp) and torch.equal(kd.cpu(), k)
+    assert torch.equal(wd.cpu().view(torch.int32), rw.view(torch.int32))
+
+
+@pytest.mark.parametrize("cap", (300, 20000, 40000))
+def test_evict_more_protected_tokens_than_the_budget(cap):
+    """Positions that do not differ: more protected tokens than fit; the lowest slots among them are kept."""
+    gen = torch.Generator().manual_seed(2)
+    w = torch.rand(1, 1, cap, generator=gen)
+    pos = torch.randint(0, 8, (1, 1, cap), generator=gen, dtype=torch.int32)
+    lens = torch.tensor([cap], dtype=torch.int32)
+    rw, rp, rn, moves = evict(w, pos, lens, lens, 100, 4, 0)
+    wd, pd, ld = _d(w, pos, lens)
+    got = kvq.evict_tokens(wd, pd, ld, ld.clone(), 100, [], sinks=4)
+    assert torch.equal(got.cpu(), rn) and torch.equal(pd.cpu(), rp) and torch.equal(wd.cpu(), rw)
+
+
 def test_evict_strided_rows_and_views():
     """Weights, positions and buffers as views of larger tensors; slots and heads outside the views keep their bytes."""
     gen = torch.Generator().manual_seed(9)

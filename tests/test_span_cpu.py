@@ -132,6 +132,13 @@ def test_evict_refusals(lib):
     e = args()
     e.bufs[0].row_bytes = 0
     assert lib.kvq_evict(C.byref(e), None) == _lib.KVQ_EINVAL
+    e = args()
+    e.bufs[0].row_bytes = (1 << 30) + 1
+    assert lib.kvq_evict(C.byref(e), None) == _lib.KVQ_ELIMIT
+    for new in (4096, 4100, 4092):                                              # overlaps the lengths that every head reads
+        e = args()
+        e.new_lengths = new
+        assert lib.kvq_evict(C.byref(e), None) == _lib.KVQ_EINVAL
 
 
 def test_wrappers_refuse_cpu_tensors():
