@@ -111,7 +111,7 @@ static int span_map(CUtensorMap* map, const KvqCacheSide& sd, const KvqAttnArgs&
 template <int FMT, bool ASYM, int GS, int D>
 static int span_box(SpanTag<FMT, ASYM, GS, D>, const SpanParams& p) {
     using S = SpanShape<FMT, ASYM, GS, D>;
-    int box = S::TSW;
+    int box = S::TS;
     if (p.pg.table)
         while (box >= 16 && p.pg.page_size % box) box /= 2;
     return box >= 16 && box * (S::RB < 128 ? S::RB : 128) >= 1024 ? box : 0;

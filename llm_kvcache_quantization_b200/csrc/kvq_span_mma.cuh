@@ -56,7 +56,7 @@ struct SpanShape {
 
 struct SpanMmaParams {
     SpanParams p;
-    int box_tokens;          // tokens of one payload copy: divides TSW and the page
+    int box_tokens;          // tokens of one payload copy: divides the tile and the page
 };
 
 __device__ __forceinline__ void sts128(uint32_t addr, uint4 v) {
