@@ -18,8 +18,10 @@
 // so far, and r moves only when a logit exceeds it by e + 3: no maximum over the warp in most tiles.
 // Copies.  A CTA walks tiles of 4 x TSW tokens, TSW per warp, through a ring of slots that each hold the K, the V and the
 // scales of a tile.  One warp fetches a tile for all: payload by cp.async.bulk.tensor (128-byte rows, 128-byte swizzle; rows
-// shorter than that hold 2 or 4 tokens, longer ones come as 2 halves), scales by cp.async.bulk, one copy per page piece or
-// warp share that has a visible token, all on the slot's mbarrier.  The warp that finishes a slot last refills it, so there
+// shorter than that hold 2 or 4 tokens, longer ones come as 2 halves), one copy per page piece that has a visible token or one
+// for the tile; scales by cp.async.bulk, or 16 bytes a lane where pieces are of fewer than 64 tokens (copies of 32 to 256 bytes
+// each keep the copy engine busy: INT8 32 x 8 K in pages of 16 65 us with them, 61 without; in pages of 64 54 and 55); all on
+// the slot's mbarrier.  The warp that finishes a slot last refills it, so there
 // is no producer warp and no barrier inside a row; every warp has looked up the pages of the tile that the slot takes next by
 // then.  Waits are bounded; an expired one raises bit 0 of the error flag.
 // (Measured and not kept, INT8 32 x 8 K / INT4 16 x 8 K, 60 / 28 us before: K and V parts in slots of their own 60 / 28, with
@@ -47,6 +49,9 @@ struct SpanShape {
     static constexpr int SCT = (ASYM ? 2 : 1) * SCB;                           // scales (and zero-points) of K, or of V
     static constexpr int SLOT = 2 * TILE;                                      // payload of a slot; the scales of all slots follow
     static constexpr int SLOTS = 2;
+    // CTAs that registers have to allow on an SM: as many as shared memory has room for, but where four groups of scales per
+    // token make the fragments large three that do not spill (INT4 with zero-points, 4 x 32 K: 49.3 us; four 53.3).
+    static constexpr int CTAS = FMT == KVQ_FMT_INT4 && NG < 4 ? 4 : 3;
     static constexpr size_t smem() {
         const size_t ring = (size_t)SLOTS * (SLOT + 2 * SCT);
         const size_t red = (size_t)kSpanWarps * kHeadsPerCta * (D + 8) * 4;
@@ -69,6 +74,14 @@ __device__ __forceinline__ void sts16(uint32_t addr, unsigned short v) {
 __device__ __forceinline__ void span_bulk(uint32_t dst, const void* src, int bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+// 16 bytes by the calling thread, and its arrival on the barrier once all of its copies so far have landed
+__device__ __forceinline__ void span_cp16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void span_cp_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 __device__ __forceinline__ uint32_t span_lds32(uint32_t addr) {
@@ -97,7 +110,7 @@ __device__ __forceinline__ uint32_t span_atom_add(uint32_t addr) {
 }
 
 template <int FMT, bool ASYM, int GS, int D>
-__global__ void __launch_bounds__(kSpanWarps * 32, 4)
+__global__ void __launch_bounds__(kSpanWarps * 32, SpanShape<FMT, ASYM, GS, D>::CTAS)
 span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     using S = SpanShape<FMT, ASYM, GS, D>;
     constexpr bool F16 = S::F16, I8 = FMT == KVQ_FMT_INT8;
@@ -121,10 +134,12 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
     __shared__ float red_w[kSpanWarps][H];
     __shared__ float red_tot[H][2];
 
+    const int box = mp.box_tokens, nbox = TS / box;
+    const bool lanes = box < 64;                               // scales come 16 bytes a lane
     const uint32_t bar0 = smem_u32(&bars[0]), done0 = smem_u32(&done[0]);
     if (threadIdx.x == 0) {
         for (int s = 0; s < SLOTS; ++s) {
-            mbar_init(bar0 + 8 * s, 1);
+            mbar_init(bar0 + 8 * s, F16 || !lanes ? 1 : 33);   // the copies' bytes, and 32 lanes' scales
             done[s] = 0;
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -139,7 +154,6 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
     if (cur.left == 0 && !p.row_mode) return;                  // uniform over the CTA
     RowView v = row_view<TS>(p, cur.b);
     const float scale2 = fabsf(a.sm_scale) * kLog2e * (F16 ? 1.f : 1.f / U24);       // q carries the sign; subnormal codes
-    const int box = mp.box_tokens, nbox = TS / box;
     // ldmatrix addresses of this lane inside a slot; 16-byte chunk c of token piece `sub`: (slot + base) ^ (c << 4), plus
     // sub * SUBSTEP, plus TS * 128 for the second half of a 256-byte row
     uint32_t lk, lv;
@@ -197,7 +211,7 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
                     atomicOr(&g_span_error_flag, 2);
                     major = 0;
                 }
-                if (!F16) sbytes = min(box, p.pg.table ? box : a.max_ctx - minor) * (2 * NG) & ~15;
+                if (!F16 && !lanes) sbytes = min(box, p.pg.table ? box : a.max_ctx - minor) * (2 * NG) & ~15;
                 all = 2 * box * RB + (ASYM ? 4 : 2) * sbytes;
             }
             all = __reduce_add_sync(0xffffffffu, all);
@@ -220,6 +234,27 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
                         span_bulk(ds + SCT + SCB, (const __half*)a.v.zp + ov_, sbytes, bar);
                     }
                 }
+            }
+            if (!F16 && lanes) {
+                constexpr int CH = SCB / 16, TPC = 8 / NG; // chunks of a table, tokens of a chunk
+#pragma unroll
+                for (int c0 = 0; c0 < CH; c0 += 32) {
+                    const int tok = (c0 + lane) * TPC, pi = tok / box & 31;
+                    const bool on = __shfl_sync(0xffffffffu, (int)vis, pi) && c0 + lane < CH;
+                    const int mj = __shfl_sync(0xffffffffu, major, pi), mn = __shfl_sync(0xffffffffu, minor, pi) + tok % box;
+                    if (on) {
+                        const uint32_t ds = sb + 16 * (c0 + lane);
+                        const long long ok_ = (long long)mj * a.k.sc_stride_b + (long long)kvh * a.k.sc_stride_h + mn * NG;
+                        const long long ov_ = (long long)mj * a.v.sc_stride_b + (long long)kvh * a.v.sc_stride_h + mn * NG;
+                        span_cp16(ds, (const __half*)a.k.scale + ok_);
+                        span_cp16(ds + SCT, (const __half*)a.v.scale + ov_);
+                        if (ASYM) {
+                            span_cp16(ds + SCB, (const __half*)a.k.zp + ok_);
+                            span_cp16(ds + SCT + SCB, (const __half*)a.v.zp + ov_);
+                        }
+                    }
+                }
+                span_cp_arrive(bar);
             }
         };
         // What the copies leave out at the end of a contiguous cache, fetched with plain loads by the warp that owns the tokens:
