@@ -28,7 +28,7 @@ static size_t pad256(size_t n) { return (n + 255) & ~(size_t)255; }
 static bool span_side_ok(const KvqCacheSide& s, const KvqAttnArgs& a, bool asym) {
     if (!s.payload || (((uintptr_t)s.payload | (uintptr_t)s.pay_stride_b | (uintptr_t)s.pay_stride_h | (uintptr_t)s.pay_stride_s) & 15))
         return false;
-    if (a.format != KVQ_FMT_FP16 && !s.scale) return false;
+    if (a.format != KVQ_FMT_FP16 && (!s.scale || (((uintptr_t)s.scale | (uintptr_t)s.zp) & 1))) return false;
     return !asym || s.zp;
 }
 
@@ -127,8 +127,20 @@ static bool span_mma_side(const KvqCacheSide& s, const SpanParams& p, int rb, in
     if ((a.Hkv > 1 && s.pay_stride_h <= 0) || (major > 1 && s.pay_stride_b <= 0)) return false;
     if (s.pay_stride_s >= (1LL << 36) || s.pay_stride_h >= (1LL << 40) || s.pay_stride_b >= (1LL << 40)) return false;
     if (ng == 0) return true;
-    if (s.sc_stride_s != ng || (a.Hkv > 1 && (s.sc_stride_h & 7)) || (major > 1 && (s.sc_stride_b & 7))) return false;
-    return !(((uintptr_t)s.scale | (uintptr_t)s.zp) & 15);
+    return s.sc_stride_s == ng;
+}
+
+// Bytes, 16 at most, that all scale and zero-point rows are aligned to.
+static int span_unit(const SpanParams& p) {
+    const KvqAttnArgs& a = p.a;
+    const int major = p.pg.table ? p.pg.num_pages : a.B;
+    uintptr_t bits = 16;
+    for (const KvqCacheSide* s : {&a.k, &a.v}) {
+        bits |= (uintptr_t)s->scale | (uintptr_t)s->zp;
+        if (a.Hkv > 1) bits |= (uintptr_t)(2 * s->sc_stride_h);
+        if (major > 1) bits |= (uintptr_t)(2 * s->sc_stride_b);
+    }
+    return (int)(bits & (~bits + 1));
 }
 
 template <int FMT, bool ASYM, int GS, int D>
@@ -147,6 +159,7 @@ static int launch_span_mma(SpanTag<FMT, ASYM, GS, D> tag, const SpanParams& p, c
     SpanMmaParams mp;
     mp.p = p;
     mp.box_tokens = span_box(tag, p);
+    mp.unit = FMT == KVQ_FMT_FP16 ? 16 : span_unit(p);
     CUtensorMap kmap, vmap;
     int rc, n;
     if ((rc = span_ctas_per_sm(tag, n))) return rc;
@@ -201,11 +214,14 @@ static int span_plan(const KvqSpanAttnArgs& s, SpanPlan& pl) {
     pl.rows = (long long)a.B * p.hr;
     const long long per_row = max_visible_tiles(p, pl.ts);
     if (pl.rows * (per_row + 64) >= (1LL << 31) || pl.rows >= (1LL << 30) || a.B > 65535) return KVQ_ELIMIT;
-    // A row of at most 256 tokens is not worth cutting (no join: INT8 1 x 2 heads of 304 slots 11.9 -> 8.1 us at 200 tokens).
+    // Rows that are not cut need no join, and the next row's CTA starts while one ends.  That pays for rows of at most 256
+    // tokens, and for longer ones when there are enough to fill the chip: INT8 256 rows of 1024 tokens 26 -> 21 us, 1024 rows of
+    // 2048 106 -> 100 (of 1 to 2048: 75 -> 61); against it, 64 rows of 1024 tokens 11.6 -> 15.9, 256 of 4096 56 -> 63.
+    const long long tokens = per_row * pl.ts;
+    p.row_mode = tokens <= 256 || (2 * pl.rows >= slots && tokens <= 1024) || (pl.rows >= 2 * slots && tokens <= 2048);
     // Otherwise a CTA has at least one tile (the generic kernel: one for each warp), and the cut counts the work of starting
     // a row (q, lookups, writing the part) as one more tile, on long rows only: of short ones it would leave CTAs idle.
     // INT8 32 x 8 K, 148 x 3 CTAs: 60.4 us without it, 57.8 with; INT4 with zero-points 1 x 1.2 K tokens 11.4 without, 13.4.
-    p.row_mode = per_row * pl.ts <= 256;
     p.row_cost = p.row_mode ? 0 : pl.kind ? (per_row >= 16 ? 1 : 0) : 4;
     p.min_tiles = (pl.kind ? 1 : 4) + p.row_cost;
     long long ctas = (pl.rows * (per_row + p.row_cost) + p.min_tiles - 1) / p.min_tiles;

@@ -13,6 +13,10 @@
 //         rounding).  V codes enter with their offset as well; offset x sum P scale_v (one mma with a matrix of ones) is
 //         taken out after every tile, so that a sum over 10^5 tokens does not carry it along.  V zero-points are one more
 //         mma, with the groups on M.
+// The sums of products with subnormal codes are exact to about 2^-14 of the largest p scale_v of 16 tokens in units of 2^-24:
+// the tensor core aligns a product by the exponents of its operands, which for a subnormal one is that of 2^-14.  That is
+// 2^-14 of an INT8 step; INT4 codes enter the product with V as 16 n, 2^-18 of a step (as n 2^-24 a channel whose heaviest
+// tokens have code 0 was off by more than the rounding of P allows).
 // Both roundings of P are relative as long as P scale_v stays in fp16's normal range, whatever the scales: probabilities are
 // 2^(x - r) with r = (a maximum of the logits x so far) - e, where e keeps 2^(e+3) scale_v <= 2^15 for the largest scale met
 // so far, and r moves only when a logit exceeds it by e + 3: no maximum over the warp in most tiles.
@@ -62,6 +66,7 @@ struct SpanShape {
 struct SpanMmaParams {
     SpanParams p;
     int box_tokens;          // tokens of one payload copy: divides the tile and the page
+    int unit;                // bytes that all scale rows are aligned to: 16, 8, 4 or 2
 };
 
 __device__ __forceinline__ void sts128(uint32_t addr, uint4 v) {
@@ -76,12 +81,14 @@ __device__ __forceinline__ void span_bulk(uint32_t dst, const void* src, int byt
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
-// 16 bytes by the calling thread, and its arrival on the barrier once all of its copies so far have landed
-__device__ __forceinline__ void span_cp16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+// by the calling thread; 2 bytes are waited for
+__device__ __forceinline__ void span_cp_small(uint32_t dst, const void* src, int unit) {
+    if (unit == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+    else if (unit == 4) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+    else sts16(dst, __ldg((const unsigned short*)src));
 }
-__device__ __forceinline__ void span_cp_arrive(uint32_t bar) {
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+__device__ __forceinline__ void span_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 __device__ __forceinline__ uint32_t span_lds32(uint32_t addr) {
@@ -135,7 +142,8 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
     __shared__ float red_tot[H][2];
 
     const int box = mp.box_tokens, nbox = TS / box;
-    const bool lanes = box < 64;                               // scales come 16 bytes a lane
+    const int unit = mp.unit;
+    const bool lanes = box < 64 || unit < 16;                  // scales come `unit` bytes a lane
     const uint32_t bar0 = smem_u32(&bars[0]), done0 = smem_u32(&done[0]);
     if (threadIdx.x == 0) {
         for (int s = 0; s < SLOTS; ++s) {
@@ -172,8 +180,7 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
         return x + sub * SUBSTEP + (RB > 128 ? (c >> 3) * (TS * 128) : 0);
     };
     // where the cache view ends, if the copies leave something of its last tokens out
-    constexpr int PER = TPR > 8 / NG ? TPR : 8 / NG;           // tokens that fill a row and 16 bytes of scales
-    const int tail = F16 || p.pg.table || a.max_ctx % PER == 0 ? -1 : a.max_ctx;
+    const int tail = !F16 && !p.pg.table && (a.max_ctx % TPR || (a.max_ctx * NG & ((unit >> 1) - 1))) ? a.max_ctx : -1;
     int slot = 0;
     uint32_t phase = 0;
     bool failed = false;
@@ -235,7 +242,29 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
                     }
                 }
             }
-            if (!F16 && lanes) {
+            if (!F16 && lanes && unit < 16) {
+                // rows of a contiguous cache whose slots do not fill 16 bytes of scales (what is left at its end: see patch())
+                const int n = a.max_ctx * NG;
+#pragma unroll 4
+                for (int c0 = 0; c0 < SCB / unit; c0 += 32) {
+                    const int el = (c0 + lane) * (unit >> 1), pi = el / NG / box & 31;
+                    const bool on = __shfl_sync(0xffffffffu, (int)vis, pi) && c0 + lane < SCB / unit;
+                    const int mj = __shfl_sync(0xffffffffu, major, pi), mn = __shfl_sync(0xffffffffu, minor, pi) * NG + el - pi * box * NG;
+                    if (on && (p.pg.table || mn + (unit >> 1) <= n)) {
+                        const uint32_t ds = sb + 2 * el;
+                        const long long ok_ = (long long)mj * a.k.sc_stride_b + (long long)kvh * a.k.sc_stride_h + mn;
+                        const long long ov_ = (long long)mj * a.v.sc_stride_b + (long long)kvh * a.v.sc_stride_h + mn;
+                        span_cp_small(ds, (const __half*)a.k.scale + ok_, unit);
+                        span_cp_small(ds + SCT, (const __half*)a.v.scale + ov_, unit);
+                        if (ASYM) {
+                            span_cp_small(ds + SCB, (const __half*)a.k.zp + ok_, unit);
+                            span_cp_small(ds + SCT + SCB, (const __half*)a.v.zp + ov_, unit);
+                        }
+                    }
+                }
+                if (unit == 2) span_arrive(bar);
+                else cp_async_mbar_arrive(bar);
+            } else if (!F16 && lanes) {
                 constexpr int CH = SCB / 16, TPC = 8 / NG; // chunks of a table, tokens of a chunk
 #pragma unroll
                 for (int c0 = 0; c0 < CH; c0 += 32) {
@@ -246,19 +275,19 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
                         const uint32_t ds = sb + 16 * (c0 + lane);
                         const long long ok_ = (long long)mj * a.k.sc_stride_b + (long long)kvh * a.k.sc_stride_h + mn * NG;
                         const long long ov_ = (long long)mj * a.v.sc_stride_b + (long long)kvh * a.v.sc_stride_h + mn * NG;
-                        span_cp16(ds, (const __half*)a.k.scale + ok_);
-                        span_cp16(ds + SCT, (const __half*)a.v.scale + ov_);
+                        cp_async16(ds, (const __half*)a.k.scale + ok_, 16);
+                        cp_async16(ds + SCT, (const __half*)a.v.scale + ov_, 16);
                         if (ASYM) {
-                            span_cp16(ds + SCB, (const __half*)a.k.zp + ok_);
-                            span_cp16(ds + SCT + SCB, (const __half*)a.v.zp + ov_);
+                            cp_async16(ds + SCB, (const __half*)a.k.zp + ok_, 16);
+                            cp_async16(ds + SCT + SCB, (const __half*)a.v.zp + ov_, 16);
                         }
                     }
                 }
-                span_cp_arrive(bar);
+                cp_async_mbar_arrive(bar);
             }
         };
         // What the copies leave out at the end of a contiguous cache, fetched with plain loads by the warp that owns the tokens:
-        // a last 128-byte row that the cache does not fill (it lies outside the tensor map) and scales that do not fill 16 bytes.
+        // a last 128-byte row that the cache does not fill (it lies outside the tensor map) and scales that do not fill a unit.
         auto patch = [&](const KvqCacheSide& cs, uint32_t dst, uint32_t sdst, int tok0) {
             const int whole = a.max_ctx / TPR * TPR, rest = a.max_ctx - whole;
             constexpr int CPT = RB / 16;
@@ -268,7 +297,7 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
                                                                 (long long)kvh * cs.pay_stride_h + (long long)tk * RB + 16 * c);
                 sts128(dst + row_ * 128 + ((cc ^ (row_ & 7)) << 4), w);
             }
-            const int swhole = a.max_ctx * NG & ~7, srest = a.max_ctx * NG - swhole;          // fp16 values
+            const int swhole = a.max_ctx * NG & -(unit >> 1), srest = a.max_ctx * NG - swhole;          // fp16 values
             if (lane < srest) {
                 const long long off = (long long)b * cs.sc_stride_b + (long long)kvh * cs.sc_stride_h + swhole + lane;
                 const uint32_t d = sdst + (swhole - tok0 * NG + lane) * 2;
@@ -656,11 +685,12 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
                                 mma16816(o[cc], prmt(X, 0u, 0x4240u), prmt(X, 0u, 0x4341u), prmt(Y, 0u, 0x4240u), prmt(Y, 0u, 0x4341u),
                                          pg[G][0], pg[G][1]);
                             } else {
-                                const uint32_t X = r[2 * e], Y = r[2 * e + 1], X8 = X >> 8, Y8 = Y >> 8;
+                                // both nibbles as 16 n: the sums of n 2^-24 keep 4 bits less
+                                constexpr uint32_t M = 0x00F000F0u;
+                                const uint32_t X = r[2 * e], Y = r[2 * e + 1];
                                 const int G = 32 * cc / GS;
-                                mma16816(o[2 * cc], X & 0x00F000F0u, X & 0x000F000Fu, Y & 0x00F000F0u, Y & 0x000F000Fu, pg[G][0], pg[G][1]);
-                                mma16816(o[2 * cc + 1], X8 & 0x00F000F0u, X8 & 0x000F000Fu, Y8 & 0x00F000F0u, Y8 & 0x000F000Fu, pg[G][0],
-                                         pg[G][1]);
+                                mma16816(o[2 * cc], X & M, (X << 4) & M, Y & M, (Y << 4) & M, pg[G][0], pg[G][1]);
+                                mma16816(o[2 * cc + 1], (X >> 8) & M, (X >> 4) & M, (Y >> 8) & M, (Y >> 4) & M, pg[G][0], pg[G][1]);
                             }
                         }
                     }
@@ -670,9 +700,9 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
 #pragma unroll
                     for (int i = 0; i < D / 16; ++i) {
                         const int G = 16 * i / GS;
-                        const float c0 = I8 ? OFFSET * U24 : 16.f * OFFSET * U24, c1 = OFFSET * U24;   // high nibbles count 16-fold
-                        o[i][0] = fmaf(sp[G][0], -c0, o[i][0]); o[i][1] = fmaf(sp[G][1], -c0, o[i][1]);
-                        o[i][2] = fmaf(sp[G][0], -c1, o[i][2]); o[i][3] = fmaf(sp[G][1], -c1, o[i][3]);
+                        const float c = I8 ? OFFSET * U24 : 16.f * OFFSET * U24;
+                        o[i][0] = fmaf(sp[G][0], -c, o[i][0]); o[i][1] = fmaf(sp[G][1], -c, o[i][1]);
+                        o[i][2] = fmaf(sp[G][0], -c, o[i][2]); o[i][3] = fmaf(sp[G][1], -c, o[i][3]);
                     }
                 }
             }
@@ -711,7 +741,7 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
             ra[(2 * t) * DR + D + g] = oz[0];
             ra[(2 * t + 1) * DR + D + g] = oz[1];
         }
-        constexpr float f0 = F16 ? 1.f : I8 ? 1.f / U24 : 1.f / (16.f * U24), f1 = F16 ? 1.f : 1.f / U24;
+        constexpr float f0 = F16 ? 1.f : I8 ? 1.f / U24 : 1.f / (16.f * U24);
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
             int d0, d1;                                        // channels of fragment rows g and g + 8
@@ -720,8 +750,8 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
             else { d0 = 32 * (i >> 1) + 4 * g + 2 * (i & 1); d1 = d0 + 1; }
             ra[(2 * t) * DR + d0] = o[i][0] * f0;
             ra[(2 * t + 1) * DR + d0] = o[i][1] * f0;
-            ra[(2 * t) * DR + d1] = o[i][2] * f1;
-            ra[(2 * t + 1) * DR + d1] = o[i][3] * f1;
+            ra[(2 * t) * DR + d1] = o[i][2] * f0;
+            ra[(2 * t + 1) * DR + d1] = o[i][3] * f0;
         }
         __syncthreads();
         if (threadIdx.x < H) {

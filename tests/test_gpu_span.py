@@ -369,6 +369,34 @@ def test_paged_append_static_scales_strided_sources_and_bad_pages(T):
         assert torch.equal(a[rest], pk[rest]) and torch.equal(b_[rest], sk[rest])
 
 
+@pytest.mark.parametrize("fmt", FORMATS[1:])
+@pytest.mark.parametrize("D,gs", ((128, 128), (128, 64), (128, 32), (64, 64), (64, 32)))
+@pytest.mark.parametrize("S,off", ((1301, 0), (1302, 0), (1304, 0), (1300, 1), (1296, 2), (333, 4)))
+def test_scale_rows_of_every_alignment(S, off, D, gs, fmt):
+    """Contiguous caches whose scale rows start on 2 to 16 bytes, by the number of slots or as views that skip some: the
+    same kernel as for aligned ones, bit for bit (the products and their order do not depend on how scales arrive)."""
+    gen, q, k, v, ks, vs, kz, vz = _case(2, 12, 2, D, S, fmt, gs, S + off)
+    lens = [S - off, 40]
+
+    def run(pad):
+        def scales(t):
+            if t is None:
+                return None
+            wide = torch.full((2, 2, S + pad, t.shape[3]), float("nan")).half().to(DEV)
+            wide[:, :, :S] = t.to(DEV)
+            return wide[:, :, off:S]
+        kk, vv = k[:, :, off:].contiguous().to(DEV), v[:, :, off:].contiguous().to(DEV)
+        return kvq.decode_attn_window(q.to(DEV), kk, vv, scales(ks), scales(vs), torch.tensor(lens, device=DEV, dtype=torch.int32),
+                                      S, k_zp=scales(kz), v_zp=scales(vz))
+    got = run(0)
+    cut = [None if t is None else t[:, :, off:] for t in (k, v, ks, vs, kz, vz)]
+    ref, tol, _, _ = attention(q, *cut, lens, S, 0)
+    check(got, ref, tol, f"{fmt} S={S} off={off}")
+    assert torch.equal(run(0), got)
+    if off == 0:
+        assert torch.equal(run(-S % 8), got)                # rows on 16 bytes
+
+
 # ------------------------------------------------------------------------------------------------ eviction
 EVICT = [
     # B, H, cap, lengths, budget, sinks, recent, seen offset
@@ -681,3 +709,28 @@ def test_contiguous_cache_with_eviction(kind):
                 assert set(range(sinks)) <= have and set(range(seen - recent, seen)) <= have and len(have) == budget
     c.clear()
     assert c.get_tokens_seen() == 0
+
+
+@pytest.mark.parametrize("fmt", ("fp16", "int8", "int4z"))
+@pytest.mark.parametrize("S", (256, 257, 1024, 1025, 2048, 2049))
+def test_many_rows_around_the_lengths_that_are_cut(S, fmt):
+    """1024 rows (more than the chip takes at once) and 256 of them; ragged, with empty ones; with weights too."""
+    B, Hq, Hkv, D = 128, 16, 8, 64
+    gen, q, k, v, ks, vs, kz, vz = _case(2, Hq, Hkv, D, S, fmt, 64, S)
+    lens = [S if b % 5 == 0 else (b * 97) % S for b in range(B)]
+    rep = [None if t is None else t.to(DEV).repeat_interleave(B // 2, 0) for t in (q, k, v, ks, vs, kz, vz)]
+    lend = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    got = kvq.decode_attn_window(rep[0], *rep[1:5], lend, S, k_zp=rep[5], v_zp=rep[6])
+    few = kvq.decode_attn_window(rep[0][:32].contiguous(), *[None if t is None else t[:32].contiguous() for t in rep[1:5]],
+                                 lend[:32].contiguous(), S, k_zp=None if kz is None else rep[5][:32].contiguous(),
+                                 v_zp=None if vz is None else rep[6][:32].contiguous())
+    w = torch.zeros(B, Hkv, S, device=DEV)
+    kvq.decode_attn_weights(rep[0], *rep[1:5], lend, w, k_zp=rep[5], v_zp=rep[6])
+    for b in (0, 1, 2, 5, 31, 64, 100, 127):
+        i = b // (B // 2)
+        one = [None if t is None else t[i:i + 1] for t in (q, k, v, ks, vs, kz, vz)]
+        ref, tol, rw, wtol = attention(*one, [lens[b]])
+        check(got[b:b + 1], ref, tol, f"{fmt} row {b}")
+        if b < 32:
+            check(few[b:b + 1], ref, tol, f"{fmt} row {b} of few")
+        assert ((w[b:b + 1].double().cpu() - rw).abs() <= wtol + 2.0 ** -22).all()
