@@ -45,7 +45,7 @@ struct SpanShape {
     static constexpr bool F16 = FMT == KVQ_FMT_FP16;
     static constexpr int RB = F16 ? 2 * D : FMT == KVQ_FMT_INT8 ? D : D / 2;   // payload bytes of a token
     static constexpr int TPR = RB < 128 ? 128 / RB : 1;                        // tokens per 128-byte row
-    static constexpr int TSW = RB >= 256 ? 16 : RB >= 64 ? 32 : 64;            // tokens of a warp
+    static constexpr int TSW = RB >= 256 ? 16 : RB >= 128 ? 32 : 64;           // tokens of a warp
     static constexpr int TS = kSpanWarps * TSW;                                // tokens of a tile
     static constexpr int NG = F16 ? 1 : D / GS;
     static constexpr int TILE = TS * RB;                                       // bytes of K (or V) of a tile
@@ -53,9 +53,10 @@ struct SpanShape {
     static constexpr int SCT = (ASYM ? 2 : 1) * SCB;                           // scales (and zero-points) of K, or of V
     static constexpr int SLOT = 2 * TILE;                                      // payload of a slot; the scales of all slots follow
     static constexpr int SLOTS = 2;
-    // CTAs that registers have to allow on an SM: as many as shared memory has room for, but where four groups of scales per
-    // token make the fragments large three that do not spill (INT4 with zero-points, 4 x 32 K: 49.3 us; four 53.3).
-    static constexpr int CTAS = FMT == KVQ_FMT_INT4 && NG < 4 ? 4 : 3;
+    // CTAs that registers have to allow on an SM: as many as shared memory has room for.
+    // (INT4 4 x 32 K with zero-points / 16 x 8 K: 32 tokens a warp and 3 or 4 CTAs 54 / 26.6 us, 64 tokens 46.6 / 24.4; a window of
+    // 16 K in 32-channel groups, one sequence: 3 CTAs 14.8 us, 2 12.4.  INT8 of 64 channels, 16 x 8 K: 39 -> 31.6.)
+    static constexpr int CTAS = RB == 32 ? 4 : RB == 64 && NG == 4 ? 2 : 3;
     static constexpr size_t smem() {
         const size_t ring = (size_t)SLOTS * (SLOT + 2 * SCT);
         const size_t red = (size_t)kSpanWarps * kHeadsPerCta * (D + 8) * 4;
