@@ -147,7 +147,7 @@ template <int FMT, bool ASYM, int GS, int D>
 static bool span_mma_ok(SpanTag<FMT, ASYM, GS, D> tag, const SpanParams& p) {
     using S = SpanShape<FMT, ASYM, GS, D>;
     const KvqAttnArgs& a = p.a;
-    if (getenv("KVQ_FORCE_GENERIC") || a.max_ctx < S::TPR) return false;
+    if (getenv("KVQ_FORCE_GENERIC") || a.max_ctx < S::TPR || a.max_ctx > (1 << 28)) return false;    // slots x groups in 32 bits
     if (!(fabsf(a.sm_scale) > 0.f && fabsf(a.sm_scale) <= 1e30f)) return false;      // masked logits are -inf before the scale
     const int ng = S::F16 ? 0 : S::NG;
     return span_box(tag, p) && span_mma_side(a.k, p, S::RB, S::TPR, ng) && span_mma_side(a.v, p, S::RB, S::TPR, ng);

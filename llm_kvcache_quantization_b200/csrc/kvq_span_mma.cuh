@@ -9,25 +9,28 @@
 //         afterwards.  Codes, q and products are exact; the offset costs one more bit of the fp32 sums.
 //         Zero-points add z_group sum_group q.
 //   P.V   channels on M, heads on N, tokens on K.  The V scale goes into P: for one group per token in fp32 before P is
-//         rounded to fp16 (one rounding, 2^-11 of p), for several groups as a product of fp16 pairs per group (a second
-//         rounding).  V codes enter with their offset as well; offset x sum P scale_v (one mma with a matrix of ones) is
+//         rounded to fp16 (one rounding, 2^-11 of p), for several groups as an fma of fp16 pairs per group, with P in two
+//         fp16 parts (rounded once too: with P in one part, rounded again by the product, INT4 outputs were off by 3.4e-4 rms, now 2.9e-4).  V codes enter with their offset as well; offset x sum P scale_v (one mma with a matrix of ones) is
 //         taken out after every tile, so that a sum over 10^5 tokens does not carry it along.  V zero-points are one more
 //         mma, with the groups on M.
 // The sums of products with subnormal codes are exact to about 2^-14 of the largest p scale_v of 16 tokens in units of 2^-24:
 // the tensor core aligns a product by the exponents of its operands, which for a subnormal one is that of 2^-14.  That is
 // 2^-14 of an INT8 step; INT4 codes enter the product with V as 16 n, 2^-18 of a step (as n 2^-24 a channel whose heaviest
 // tokens have code 0 was off by more than the rounding of P allows).
-// Both roundings of P are relative as long as P scale_v stays in fp16's normal range, whatever the scales: probabilities are
+// The rounding of P is relative as long as P scale_v stays in fp16's normal range, whatever the scales: probabilities are
 // 2^(x - r) with r = (a maximum of the logits x so far) - e, where e keeps 2^(e+3) scale_v <= 2^15 for the largest scale met
 // so far, and r moves only when a logit exceeds it by e + 3: no maximum over the warp in most tiles.
 // Copies.  A CTA walks tiles of 4 x TSW tokens, TSW per warp, through a ring of slots that each hold the K, the V and the
 // scales of a tile.  One warp fetches a tile for all: payload by cp.async.bulk.tensor (128-byte rows, 128-byte swizzle; rows
 // shorter than that hold 2 or 4 tokens, longer ones come as 2 halves), one copy per page piece that has a visible token or one
 // for the tile; scales by cp.async.bulk, or 16 bytes a lane where pieces are of fewer than 64 tokens (copies of 32 to 256 bytes
-// each keep the copy engine busy: INT8 32 x 8 K in pages of 16 65 us with them, 61 without; in pages of 64 54 and 55); all on
-// the slot's mbarrier.  The warp that finishes a slot last refills it, so there
-// is no producer warp and no barrier inside a row; every warp has looked up the pages of the tile that the slot takes next by
-// then.  Waits are bounded; an expired one raises bit 0 of the error flag.
+// each keep the copy engine busy: INT8 32 x 8 K in pages of 16 65 us with them, 61 without; in pages of 64 54 and 55) or of
+// contiguous rows that do not start on 16 bytes; all on the slot's mbarrier.  The warp that finishes a slot last refills it, so
+// there is no producer warp and no barrier inside a row; every warp has looked up the pages of the tile that the slot takes
+// next by then.  Waits are bounded; an expired one raises bit 0 of the error flag.
+// Measured: INT8 32 x 8 K 52 us (5.2 TB/s), pages of 64 55, of 16 61; INT4 16 x 8 K 24.4 (2.8 TB/s); INT4 with zero-points and
+// 32-channel groups 4 x 32 K 48.8 (3.4 TB/s), pages of 32 62; fp16 16 x 4 K 28.4 (4.7 TB/s).  INT8 and fp16 are bound by HBM with
+// two slots per CTA in flight, INT4 by instructions (some 500 of 32 tokens and a warp, a third of them unpacking).
 // (Measured and not kept, INT8 32 x 8 K / INT4 16 x 8 K, 60 / 28 us before: K and V parts in slots of their own 60 / 28, with
 // 8 KB slots 64 / 36; a ring per warp 62 / 35.)
 #pragma once
@@ -54,7 +57,7 @@ struct SpanShape {
     static constexpr int SLOT = 2 * TILE;                                      // payload of a slot; the scales of all slots follow
     static constexpr int SLOTS = 2;
     // CTAs that registers have to allow on an SM: as many as shared memory has room for.
-    // (INT4 4 x 32 K with zero-points / 16 x 8 K: 32 tokens a warp and 3 or 4 CTAs 54 / 26.6 us, 64 tokens 46.6 / 24.4; a window of
+    // (INT4 4 x 32 K with zero-points / 16 x 8 K: 32 tokens a warp and 3 or 4 CTAs 54 / 26.6 us, 64 tokens 47 / 24.4; a window of
     // 16 K in 32-channel groups, one sequence: 3 CTAs 14.8 us, 2 12.4.  INT8 of 64 channels, 16 x 8 K: 39 -> 31.6.)
     static constexpr int CTAS = RB == 32 ? 4 : RB == 64 && NG == 4 ? 2 : 3;
     static constexpr size_t smem() {
@@ -517,6 +520,7 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
             }
             // ================= online softmax
             uint32_t pb[SUB][2];                               // P^T fragments; for NG == 1 with the V scale inside
+            uint32_t pl[!F16 && NG > 1 ? SUB : 1][2];          // what rounding to fp16 left of P; for several groups
             uint32_t pz[ASYM && NG == 1 ? SUB : 1][2];         // P^T without the scale, for the zero-points
             const uint32_t vb = ring_u + slot * SLOT + TILE, vsb = scale_u + slot * 2 * SCT + SCT + warp * TSW * NG * 2, vzb = vsb + SCB;
             if (active) {
@@ -623,8 +627,14 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
                         load_row_floats<1>(vsb + (16 * sub + 8 + g) * 2, vc);
                         p0 *= va[0]; p1 *= va[0]; p2 *= vc[0]; p3 *= vc[0];
                     }
-                    pb[sub][0] = movmatrix_trans(pack_h2(p0, p1));     // tokens 2t, 2t+1 of head g
-                    pb[sub][1] = movmatrix_trans(pack_h2(p2, p3));     // tokens 2t+8, 2t+9
+                    const uint32_t h0 = pack_h2(p0, p1), h1 = pack_h2(p2, p3);
+                    pb[sub][0] = movmatrix_trans(h0);          // tokens 2t, 2t+1 of head g
+                    pb[sub][1] = movmatrix_trans(h1);          // tokens 2t+8, 2t+9
+                    if (!F16 && NG > 1) {
+                        const float2 f0 = __half22float2(u32_as_h2(h0)), f1 = __half22float2(u32_as_h2(h1));
+                        pl[sub][0] = movmatrix_trans(pack_h2(p0 - f0.x, p1 - f0.y));
+                        pl[sub][1] = movmatrix_trans(pack_h2(p2 - f1.x, p3 - f1.y));
+                    }
                 }
                 l_run[0] += ps[0];
                 l_run[1] += ps[1];
@@ -653,8 +663,8 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
                         load_scale_pairs<NG>(vsb + (16 * sub + 2 * t + 8) * 2 * NG, sy, 0xffffffffu);
 #pragma unroll
                         for (int G = 0; G < NG; ++G) {
-                            pg[G][0] = hmul2_u(pb[sub][0], sx[G]);
-                            pg[G][1] = hmul2_u(pb[sub][1], sy[G]);
+                            pg[G][0] = hfma2_u(pb[sub][0], sx[G], hmul2_u(pl[sub][0], sx[G]));
+                            pg[G][1] = hfma2_u(pb[sub][1], sy[G], hmul2_u(pl[sub][1], sy[G]));
                         }
                     }
                     constexpr uint32_t kOnes = 0x3c003c00u;
@@ -672,6 +682,7 @@ span_mma_kernel(const SpanMmaParams mp, const __grid_constant__ CUtensorMap kmap
                         }
                         const int zs = ASYM && NG == 1 ? sub : 0;
                         mma16816(oz, zlo, 0u, zhi, 0u, NG == 1 ? pz[zs][0] : pb[sub][0], NG == 1 ? pz[zs][1] : pb[sub][1]);
+                        if (NG > 1) mma16816(oz, zlo, 0u, zhi, 0u, pl[sub][0], pl[sub][1]);
                     }
 #pragma unroll
                     for (int c = 0; c < RB / 16; c += 2) {
