@@ -683,6 +683,7 @@ def span_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: Option
         window = 0
     elif window < 1 or sinks < 0:
         raise ValueError(f"window must be >= 1 and sinks >= 0, got {window}, {sinks}")
+    window, sinks = min(int(window), 2 ** 31 - 1), min(int(sinks), 2 ** 31 - 1)     # no row is longer
     s = _lib.KvqSpanAttnArgs()
     a = s.attn
     if block_table is None:
@@ -720,7 +721,7 @@ def span_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: Option
         raise ValueError("a paged cache needs context_lens")
     a.k = _cache_side(k, k_scale, k_zp, None)
     a.v = _cache_side(v, v_scale, v_zp, None)
-    s.window, s.sinks = int(window), int(sinks)
+    s.window, s.sinks = window, sinks
     if weights is not None:
         if weights.dtype != torch.float32 or weights.ndim != 3 or weights.shape[:2] != (B, Hkv) or weights.shape[2] < span:
             raise ValueError(f"weights must be fp32 [B={B}, Hkv={Hkv}, >= {span}], got {weights.dtype} {tuple(weights.shape)}")
@@ -857,6 +858,8 @@ def evict(weights: torch.Tensor, positions: torch.Tensor, lengths: torch.Tensor,
     budget, sinks, recent = int(budget), int(sinks), int(recent)
     if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
         raise ValueError(f"need budget >= 1 and 0 <= sinks + recent <= budget, got {budget}, {sinks}, {recent}")
+    if budget >= 2 ** 31:
+        raise ValueError(f"budget must be less than 2^31, got {budget}")
     if len(buffers) > _lib.EVICT_MAX_BUFS:
         raise ValueError(f"at most {_lib.EVICT_MAX_BUFS} buffers, got {len(buffers)}")
     e = _lib.KvqEvictArgs()

@@ -1,4 +1,5 @@
 """CPU-side checks of the bounded and paged cache operators: refusals before any launch, and the page bookkeeping."""
+import contextlib
 import ctypes as C
 
 import pytest
@@ -260,6 +261,33 @@ def test_evict_argument_checks(no_device_check):
                       (dict(w=w[:, :1].expand(2, 2, 8)), "rows that do not overlap")):
         with pytest.raises(ValueError, match=match):
             ev(**kw)
+
+
+def test_numbers_beyond_32_bits(no_device_check, monkeypatch):
+    """A window that 32 bits do not hold is the whole row, not what is left of the number; such a budget is refused."""
+    k, ks = _pool()
+    seen = []
+
+    class Fake:
+        def kvq_span_attn_workspace_bytes(self, s):
+            return 256
+
+        def kvq_span_attn(self, s, stream):
+            seen.append((s._obj.window, s._obj.sinks))
+            return 0
+    monkeypatch.setattr(_lib, "load", lambda: Fake())
+    monkeypatch.setattr(ops, "_stream_ptr", lambda d: 0)
+    monkeypatch.setattr(ops, "_MARSHAL", type("N", (), {"span_attn": lambda *a: None})())
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    for window, sinks in ((2 ** 32 + 5, 4), (7, 2 ** 33 + 1)):
+        ops.span_attn(torch.zeros(4, 4, 128).half(), k, k, ks, ks, None, window=window, sinks=sinks)
+    assert seen == [(2 ** 31 - 1, 4), (7, 2 ** 31 - 1)]
+    w, p = torch.zeros(1, 1, 8), torch.full((1, 1, 8), -1, dtype=torch.int32)
+    n = torch.full((1,), 8, dtype=torch.int32)
+    monkeypatch.undo()
+    monkeypatch.setattr(ops, "_require_cuda", lambda *t: torch.device("cpu"))
+    with pytest.raises(ValueError, match="2.31"):
+        ops.evict(w, p, n, n, 2 ** 32 + 1, ())
 
 
 def test_plain_eviction_by_hand():
