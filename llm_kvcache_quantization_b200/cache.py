@@ -277,6 +277,8 @@ class _CacheBase:
         if self._window is not None:
             ctx = None if self._dev_positions is None else self._dev_positions[1]
             return ops.span_attn(q, k, v, ks, vs, ctx, sm_scale, window=self._window[0], sinks=self._window[1], **kw)
+        if q.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise ValueError("eviction changes the lengths on the host: a step with it cannot be captured into a CUDA graph")
         budget, sinks, recent = self._evict
         st = self._eviction_buffers(layer_id)
         res = ops.span_attn(q, k, v, ks, vs, None, sm_scale, weights=st["w"], **kw)

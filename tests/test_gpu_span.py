@@ -734,3 +734,23 @@ def test_many_rows_around_the_lengths_that_are_cut(S, fmt):
         if b < 32:
             check(few[b:b + 1], ref, tol, f"{fmt} row {b} of few")
         assert ((w[b:b + 1].double().cpu() - rw).abs() <= wtol + 2.0 ** -22).all()
+
+
+def test_a_step_with_eviction_is_not_captured():
+    """Its lengths are the host's; the call is refused before anything is launched or kept, and works afterwards."""
+    c = kvq.INT8KVCache(1, device=DEV, group_size=32)
+    c.enable_eviction(40, 2, 8)
+    gen = torch.Generator().manual_seed(4)
+    k = torch.randn(1, 2, 50, 128, generator=gen).half().to(DEV)
+    q = torch.randn(1, 4, 128, generator=gen).half().to(DEV)
+    c.append(0, k, k)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = q + 1                                          # a graph that is not empty
+        with pytest.raises(ValueError, match="captured"):
+            c.fused_decode(0, q, 0.09)
+    assert c.get_seq_len() == 50
+    g.replay()
+    out = c.fused_decode(0, q, 0.09)
+    assert c.get_seq_len() == 40 and torch.isfinite(out).all() and torch.equal(y, q + 1)
