@@ -138,6 +138,12 @@ class PagedKVCache:
                              "appended yet")
 
     # ---- one step
+    def _not_captured(self) -> None:
+        # pages and lengths are the host's, and the tables of a step live until the next one
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise ValueError("a step of a paged cache cannot be captured into a CUDA graph: use paged_append and "
+                             "decode_attn_paged with tables of your own")
+
     def _begin(self, batch: int, tokens: int, new_lens: Optional[Sequence[int]]) -> None:
         """Reserve the pages of the step's tokens and upload its tables.  Nothing changes if the pool is too small."""
         self._between_steps("a new step")
@@ -188,6 +194,7 @@ class PagedKVCache:
             raise ValueError(f"expected [B, {self.num_kv_heads}, T, {self.head_dim}], got {tuple(k.shape)}")
         if not k.is_cuda or not v.is_cuda:
             raise ValueError("this cache quantizes with a CUDA kernel; CPU tensors are not supported")
+        self._not_captured()
         if layer_id == 0:
             self._begin(k.shape[0], k.shape[2], new_lens)
             self._step_tokens = k.shape[2]
@@ -205,6 +212,7 @@ class PagedKVCache:
 
     def _live_step(self, layer_id: int):
         pool = self._check_layer(layer_id)
+        self._not_captured()
         if self._step is None or layer_id >= self._step_layer:
             raise ValueError(f"nothing was appended to layer {layer_id} in this step")
         return pool, self._step

@@ -754,3 +754,19 @@ def test_a_step_with_eviction_is_not_captured():
     g.replay()
     out = c.fused_decode(0, q, 0.09)
     assert c.get_seq_len() == 40 and torch.isfinite(out).all() and torch.equal(y, q + 1)
+
+def test_a_step_of_a_paged_cache_is_not_captured():
+    c = kvq.PagedKVCache(1, 8, 2, 128, page_size=16, device=DEV, group_size=32)
+    c.add_sequence()
+    k = torch.randn(1, 2, 20, 128, device=DEV).half()
+    q = torch.randn(1, 4, 128, device=DEV).half()
+    c.append(0, k, k)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = q + 1
+        for call in (lambda: c.append(0, k, k), lambda: c.fused_decode(0, q), lambda: c.get_kv(0)):
+            with pytest.raises(ValueError, match="captured"):
+                call()
+    assert c.get_seq_lens() == (20,) and c.num_free_pages == 6
+    assert torch.isfinite(c.fused_decode(0, q)).all()
