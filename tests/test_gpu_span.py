@@ -755,6 +755,7 @@ def test_a_step_with_eviction_is_not_captured():
     out = c.fused_decode(0, q, 0.09)
     assert c.get_seq_len() == 40 and torch.isfinite(out).all() and torch.equal(y, q + 1)
 
+
 def test_a_step_of_a_paged_cache_is_not_captured():
     c = kvq.PagedKVCache(1, 8, 2, 128, page_size=16, device=DEV, group_size=32)
     c.add_sequence()
